@@ -375,6 +375,133 @@ int prism_gemm_bf16(int M, int N, int K, const uint16_t* A, const uint16_t* B,
 int prism_runmyh100(int M, int N, int K, const uint16_t* A, const uint16_t* B,
                     uint16_t* C, int* DB);
 
+/* --------------------------------------------------------- expert layers -- */
+/*
+ * The operators of a layer of experts: the router, the rows on their way to the
+ * experts and back, the experts' products in bf16 with their gradients, and
+ * products of a few rows with weights held in 4 bits. The reference has no
+ * counterpart (its matrix product is the dense one of
+ * examples/h100_matmul.py:20-297); the formulas are written out at each call.
+ *
+ * Shared rules. Element types are PRISM_TYPE_*; bf16 values are 16-bit
+ * patterns. ld* are the elements between rows of a row-major matrix, at least
+ * a row's length; pointers need the alignment of their elements only (bases and
+ * rows that are multiples of 16 bytes are faster). Outputs must not overlap
+ * inputs. offsets is a group table in device memory, groups + 1 entries: group
+ * g owns the rows offsets[g] .. offsets[g + 1] - 1 of the row operand (empty
+ * groups are fine); rows outside [offsets[0], offsets[groups]) are neither used
+ * nor written. Table, slot and row entries are cut to the buffers given, so
+ * wrong ones give wrong results but no access outside. Sums run in 32 bits, in
+ * an order that does not change from run to run. The calls allocate nothing,
+ * keep nothing and may be captured into HIP graphs.
+ */
+enum { PRISM_TYPE_F32 = 0, PRISM_TYPE_BF16 = 1 };
+
+/*
+ * For every token t the k largest of its logits z (tokens x experts, row
+ * stride ld, of `type`): chosen[t * k + j] the expert with the j-th largest
+ * logit (equal ones: the lower index; NaN counts as the largest; -inf is never
+ * chosen: -1 where nothing is left) and weights[t * k + j] =
+ * exp(z_j - z_0) / sum, summed over the chosen ones (renormalise != 0) or over
+ * all logits of the token; 0 for expert -1. At most 1024 experts, k <= 32.
+ */
+int prism_route_topk(const void* logits, int type, int64_t ld, int64_t tokens, int experts, int k,
+                     int renormalise, float* weights, int32_t* chosen, void* stream);
+
+/*
+ * Gradient of the weights above with respect to the logits, every element of
+ * grad_logits (of `type`, row stride ld_grad) written: with g = grad_weights
+ * and c = sum_j w_j g_j, w_j (g_j - c) for the chosen experts and 0 or (not
+ * renormalised) -c p_e for the others, p the softmax over all logits. weights
+ * and chosen are prism_route_topk's for these logits.
+ */
+int prism_route_topk_backward(const float* grad_weights, const void* logits, int type, int64_t ld,
+                              const float* weights, const int32_t* chosen, int64_t tokens, int experts,
+                              int k, int renormalise, void* grad_logits, int64_t ld_grad, void* stream);
+
+/*
+ * The plan of a choice: its tokens * k entries (t, j), numbered t k + j, in the
+ * order of their experts, equal experts in the order of the entries.
+ * offsets[e] (experts + 1 of them) = entries of experts below e, rows[s] = the
+ * entry in slot s (-1 from offsets[experts] on), slots[t * k + j] = its slot
+ * (-1 where chosen is -1 or not below `experts`). offsets is the group table of
+ * the products. The workspace (4-byte aligned, any contents, nothing kept in
+ * it) holds prism_expert_plan_workspace_bytes; calls that share one must be
+ * ordered on one stream.
+ */
+size_t prism_expert_plan_workspace_bytes(int64_t tokens, int k, int experts);
+int prism_expert_plan(const int32_t* chosen, int64_t tokens, int k, int experts, int32_t* offsets,
+                      int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
+ * out[s] = x[rows[s] / k] for the n_slots slots with rows[s] >= 0 (the others
+ * are left as they are). x: tokens x width, out: n_slots x width, both of
+ * `type`. Its gradient is prism_expert_combine with weights == NULL.
+ */
+int prism_expert_gather(const void* x, int type, int64_t ldx, int64_t tokens, int k, const int32_t* rows,
+                        void* out, int64_t ldo, int64_t n_slots, int64_t width, void* stream);
+
+/*
+ * out[t] = sum_j weights[t * k + j] y[slots[t * k + j]] over the entries with a
+ * slot (weights == NULL: all 1); zeros for a token without any. y: n_slots x
+ * width, out: tokens x width, both of `type`.
+ */
+int prism_expert_combine(const void* y, int type, int64_t ldy, int64_t n_slots, const float* weights,
+                         const int32_t* slots, int64_t tokens, int k, void* out, int64_t ldo,
+                         int64_t width, void* stream);
+
+/*
+ * Gradients of prism_expert_combine: grad_y[slots[t * k + j]] =
+ * weights[t * k + j] grad_out[t] (slots of no entry are left as they are) and
+ * grad_weights[t * k + j] = <grad_out[t], y[slots[t * k + j]]> (0 without a
+ * slot). An entry's slot must be its own: two entries with one slot race.
+ */
+int prism_expert_combine_backward(const void* grad_out, int type, int64_t ld_grad, const void* y,
+                                  int64_t ldy, const float* weights, const int32_t* slots,
+                                  int64_t tokens, int k, void* grad_y, int64_t ld_grad_y,
+                                  float* grad_weights, int64_t n_slots, int64_t width, void* stream);
+
+/*
+ * prism_gemm_bf16 group by group: D[r] = A[r] @ B[g]^T for the rows r of group
+ * g. A: rows x K, B: groups matrices N x K, group_stride elements apart, D:
+ * rows x N of d_type; any sizes.
+ */
+int prism_gemm_bf16_grouped(int groups, int64_t rows, int N, int K, const uint16_t* A, int64_t lda,
+                            const uint16_t* B, int64_t ldb, int64_t group_stride, const int32_t* offsets,
+                            void* D, int64_t ldd, int d_type, void* stream);
+
+/* Its gradient for A: dA[r] = dD[r] @ B[g]. dD: rows x N, dA: rows x K of a_type. */
+int prism_gemm_bf16_grouped_grad_a(int groups, int64_t rows, int N, int K, const uint16_t* dD,
+                                   int64_t ldd, const uint16_t* B, int64_t ldb, int64_t group_stride,
+                                   const int32_t* offsets, void* dA, int64_t lda, int a_type,
+                                   void* stream);
+
+/*
+ * Its gradient for B: dB[g] = the sum over the rows r of group g of
+ * dD[r]^T A[r] (zeros for an empty group: every element of dB is written), of
+ * b_type, matrices group_stride elements apart.
+ */
+int prism_gemm_bf16_grouped_grad_b(int groups, int64_t rows, int N, int K, const uint16_t* dD,
+                                   int64_t ldd, const uint16_t* A, int64_t lda, const int32_t* offsets,
+                                   void* dB, int64_t ldb, int64_t group_stride, int b_type, void* stream);
+
+/*
+ * A few rows times weights held in 4 bits: y[r][n] = sum_k x[r][k]
+ * scales[n][k / group_size] (q[n][k] - zeros[n][k / group_size]) for the rows of
+ * group g and its matrix. x: rows x K bf16 (finite: an infinity gives NaN). q: groups matrices of N rows
+ * of (K + 1) / 2 bytes, two weights to a byte, the even k in the low nibble; ldq
+ * and group_stride in bytes. scales (bf16) and zeros (uint8, NULL: 8
+ * throughout): groups x N x ceil(K / group_size), contiguous; group_size a
+ * multiple of 32. offsets may be NULL for one matrix: all rows use it. y: rows x
+ * N of y_type. Made for up to 16 rows a group, which cost what one costs; more
+ * are right, and read the weights once per 64 rows.
+ */
+int prism_gemv_w4(int groups, int64_t rows, int N, int K, const uint16_t* x, int64_t ldx,
+                  const uint8_t* q, int64_t ldq, int64_t group_stride, const uint16_t* scales,
+                  const uint8_t* zeros, int group_size, const int32_t* offsets, void* y, int64_t ldy,
+                  int y_type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

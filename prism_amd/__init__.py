@@ -1,7 +1,7 @@
 """prism_amd: MI355X (gfx950) kernels for the data-parallel path of manya-bansal/prism.
 
 Hand-written HIP kernels (add_m, single-pass look-back scan, the fp32 SGEMM
-progression, a bf16 MFMA GEMM) behind a C-ABI shared library
+progression, a bf16 MFMA GEMM, the operators of a layer of experts) behind a C-ABI shared library
 (include/prism_amd.h), with this package as the ctypes-level host mirror of the
 reference's launchers. Importing the package does not touch the GPU; the first
 call loads (and, if the file is absent, builds) libprism_amd.so.
@@ -28,6 +28,20 @@ from .ops import (  # noqa: F401
     sgemm_workspace_size,
     tile_coords,
     wave_regroup,
+)
+from .experts import (  # noqa: F401
+    Routing,
+    expert_combine,
+    expert_combine_backward,
+    expert_gather,
+    expert_gather_backward,
+    expert_plan,
+    gemm_bf16_grouped,
+    gemm_bf16_grouped_grad_a,
+    gemm_bf16_grouped_grad_b,
+    gemv_w4,
+    route_topk,
+    route_topk_backward,
 )
 
 __version__ = "0.1.0"

@@ -176,4 +176,65 @@ int prism_runmyh100(int M, int N, int K, const uint16_t* A, const uint16_t* B, u
     return launch_gemm_bf16(M, N, K, A, B, nullptr, C, nullptr);
 }
 
+static_assert(PRISM_TYPE_F32 == kTypeF32 && PRISM_TYPE_BF16 == kTypeBf16, "include/prism_amd.h and common.h disagree");
+
+int prism_gemm_bf16_grouped(int groups, int64_t rows, int N, int K, const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb,
+                            int64_t group_stride, const int32_t* offsets, void* D, int64_t ldd, int d_type, void* stream) {
+    return launch_gemm_grouped(GroupedForm::kForward, groups, rows, N, K, A, lda, B, ldb, group_stride, offsets, D, ldd, d_type,
+                               static_cast<hipStream_t>(stream));
+}
+
+int prism_gemm_bf16_grouped_grad_a(int groups, int64_t rows, int N, int K, const uint16_t* dD, int64_t ldd, const uint16_t* B, int64_t ldb,
+                                   int64_t group_stride, const int32_t* offsets, void* dA, int64_t lda, int a_type, void* stream) {
+    return launch_gemm_grouped(GroupedForm::kGradA, groups, rows, N, K, dD, ldd, B, ldb, group_stride, offsets, dA, lda, a_type,
+                               static_cast<hipStream_t>(stream));
+}
+
+int prism_gemm_bf16_grouped_grad_b(int groups, int64_t rows, int N, int K, const uint16_t* dD, int64_t ldd, const uint16_t* A, int64_t lda,
+                                   const int32_t* offsets, void* dB, int64_t ldb, int64_t group_stride, int b_type, void* stream) {
+    return launch_gemm_grouped(GroupedForm::kGradB, groups, rows, N, K, dD, ldd, A, lda, group_stride, offsets, dB, ldb, b_type,
+                               static_cast<hipStream_t>(stream));
+}
+
+int prism_gemv_w4(int groups, int64_t rows, int N, int K, const uint16_t* x, int64_t ldx, const uint8_t* q, int64_t ldq, int64_t group_stride,
+                  const uint16_t* scales, const uint8_t* zeros, int group_size, const int32_t* offsets, void* y, int64_t ldy, int y_type, void* stream) {
+    return launch_gemv_w4(groups, rows, N, K, x, ldx, q, ldq, group_stride, scales, zeros, group_size, offsets, y, ldy, y_type,
+                          static_cast<hipStream_t>(stream));
+}
+
+int prism_route_topk(const void* logits, int type, int64_t ld, int64_t tokens, int experts, int k, int renormalise, float* weights,
+                     int32_t* chosen, void* stream) {
+    return launch_route_topk(type, logits, ld, tokens, experts, k, renormalise, weights, chosen, static_cast<hipStream_t>(stream));
+}
+
+int prism_route_topk_backward(const float* grad_weights, const void* logits, int type, int64_t ld, const float* weights, const int32_t* chosen,
+                              int64_t tokens, int experts, int k, int renormalise, void* grad_logits, int64_t ld_grad, void* stream) {
+    return launch_route_backward(type, grad_weights, logits, ld, weights, chosen, tokens, experts, k, renormalise, grad_logits, ld_grad,
+                                 static_cast<hipStream_t>(stream));
+}
+
+size_t prism_expert_plan_workspace_bytes(int64_t tokens, int k, int experts) { return expert_plan_workspace_bytes(tokens, k, experts); }
+
+int prism_expert_plan(const int32_t* chosen, int64_t tokens, int k, int experts, int32_t* offsets, int32_t* rows, int32_t* slots,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+    return launch_expert_plan(chosen, tokens, k, experts, offsets, rows, slots, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int prism_expert_gather(const void* x, int type, int64_t ldx, int64_t tokens, int k, const int32_t* rows, void* out, int64_t ldo, int64_t n_slots,
+                        int64_t width, void* stream) {
+    return launch_expert_gather(type, x, ldx, tokens, k, rows, out, ldo, n_slots, width, static_cast<hipStream_t>(stream));
+}
+
+int prism_expert_combine(const void* y, int type, int64_t ldy, int64_t n_slots, const float* weights, const int32_t* slots, int64_t tokens, int k,
+                         void* out, int64_t ldo, int64_t width, void* stream) {
+    return launch_expert_sum(type, y, ldy, n_slots, weights, slots, tokens, k, out, ldo, width, static_cast<hipStream_t>(stream));
+}
+
+int prism_expert_combine_backward(const void* grad_out, int type, int64_t ld_grad, const void* y, int64_t ldy, const float* weights,
+                                  const int32_t* slots, int64_t tokens, int k, void* grad_y, int64_t ld_grad_y, float* grad_weights, int64_t n_slots,
+                                  int64_t width, void* stream) {
+    return launch_expert_sum_backward(type, grad_out, ld_grad, y, ldy, weights, slots, tokens, k, grad_y, ld_grad_y, grad_weights, n_slots, width,
+                                      static_cast<hipStream_t>(stream));
+}
+
 }  // extern "C"

@@ -87,4 +87,28 @@ int launch_sgemm_ws(int variant, int M, int N, int K, float alpha, const float* 
 int launch_gemm_bf16(int M, int N, int K, const uint16_t* A, const uint16_t* B, float* D_f32,
                      uint16_t* C_bf16_colmajor, hipStream_t s);
 
+// Element types of the expert-layer operators: the values of PRISM_TYPE_* in include/prism_amd.h.
+constexpr int kTypeF32 = 0, kTypeBf16 = 1;
+// The grouped products; (first, second, out) are (A, B, D), (dD, B, dA) or (dD, A, dB), group_stride the elements
+// between the matrices of B or dB.
+enum class GroupedForm { kForward, kGradA, kGradB };
+int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int K, const uint16_t* first, long long ld_first,
+                        const uint16_t* second, long long ld_second, long long group_stride, const int32_t* offsets, void* out,
+                        long long ld_out, int out_type, hipStream_t s);
+int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, long long ldx, const uint8_t* q, long long ldq, long long q_stride,
+                   const uint16_t* scales, const uint8_t* zeros, int group_size, const int32_t* offsets, void* y, long long ldy, int out_type, hipStream_t s);
+int launch_route_topk(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
+                      hipStream_t s);
+int launch_route_backward(int type, const float* grad, const void* logits, long long ld, const float* weights, const int32_t* chosen, long long tokens,
+                          int experts, int k, int renormalise, void* out, long long ldo, hipStream_t s);
+size_t expert_plan_workspace_bytes(long long tokens, int k, int experts);
+int launch_expert_plan(const int32_t* chosen, long long tokens, int k, int experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* ws,
+                       size_t ws_bytes, hipStream_t s);
+int launch_expert_gather(int type, const void* x, long long ldx, long long tokens, int k, const int32_t* rows, void* out, long long ldo,
+                         long long n_slots, long long width, hipStream_t s);
+int launch_expert_sum(int type, const void* y, long long ldy, long long n_slots, const float* weights, const int32_t* slots, long long tokens, int k,
+                      void* out, long long ldo, long long width, hipStream_t s);
+int launch_expert_sum_backward(int type, const void* dout, long long ldd, const void* y, long long ldy, const float* weights, const int32_t* slots,
+                               long long tokens, int k, void* dy, long long lddy, float* dw, long long n_slots, long long width, hipStream_t s);
+
 }  // namespace prism
