@@ -226,6 +226,420 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
     }
 }
 
+// ------------------------------------------------------------------------------------- many rows: 256 x 256 tiles --
+// The pipeline of gemm_bf16_early_kernel (gemm_bf16.hip) for ragged groups and turned operands: four waves of 128 x 128
+// with all 256 accumulation registers, one workgroup per CU that walks its tiles, direct-to-LDS loads into two stages of
+// 64 c, all fragments of a stage read behind the first 32 matrix instructions of its phase, a barrier in mid-phase that
+// frees the stage, the loads of the tile after next spread over the rest, and the last two phases of a tile fetching the
+// first two stages of the workgroup's next tile. What that kernel's comments say about the matrix instruction from inline
+// assembly and about scalar operands of direct loads holds here too:
+//   * an accumulator is read by nothing but that instruction within 64 clocks of its last one (grouped_settle);
+//   * a fragment register written by the vector ALU is not used by the next few instructions (s_nop at the loop's head);
+//   * descriptors and scalar offsets are in scalar registers well before the load that reads them.
+// New here: every load goes through its descriptor's extent, which ends with the group (straight: the lines that exist;
+// turned: the c that exist), so that ragged tiles need no code of their own, and the walk over the tiles of all groups
+// reads a table that the workgroup makes of the offsets in LDS at its start.
+__device__ __forceinline__ void mfma_in_place(f32x4& c, bf16x8 a, bf16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void grouped_settle() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory"); }
+
+// On the scalar ALU by name: a minimum inside a maximum becomes v_med3_i32 otherwise, and a descriptor with a word from
+// the vector ALU cannot be an operand of the load.
+__device__ __forceinline__ int scalar_min(int a, int b) {
+    int r;
+    asm("s_min_i32 %0, %1, %2" : "=s"(r) : "s"(a), "s"(b) : "scc");
+    return r;
+}
+__device__ __forceinline__ int scalar_max(int a, int b) {
+    int r;
+    asm("s_max_i32 %0, %1, %2" : "=s"(r) : "s"(a), "s"(b) : "scc");
+    return r;
+}
+
+constexpr int kBigGroups = 1024;  // groups that the table in LDS holds
+constexpr int kBigBlockM = 8;     // row tiles of a group that are walked together (see tile order below)
+
+// Behind how many of a phase's 128 matrix instructions the barrier that frees the stage sits, and the instructions
+// between two loads.
+template <int TURNED>
+struct BigPace {
+    static constexpr int kReads = 1 + (TURNED > 0), kBarrierAt = 36, kGap = 6;
+};
+
+// Register address of a fragment in LDS and how the fragment is read from it; ROW0: the wave's first line of the tile.
+template <bool TURNED>
+struct BigFragments {
+    uint32_t at[TURNED ? 8 : 2];  // byte addresses in LDS
+    __device__ __forceinline__ void init(const uint16_t* tile, int row0, int lane) {
+        const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)tile));
+        const int l16 = lane & 15, lq = lane >> 4;
+        if constexpr (!TURNED) {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) at[kk] = base + ((row0 + l16) * kBK + ((4 * kk + lq) ^ ((l16 >> 1) & 7)) * 8) * 2;
+        } else {
+            const int row = 8 * lq + (l16 >> 2), f = (row & 3) | ((row & 8) >> 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) at[i] = base + (row * 256 + ((row0 / 16 + i) ^ f) * 16 + 4 * (l16 & 3)) * 2;
+        }
+        // As they are from here on: taken apart into a constant and the rest, the constant parts of the reads no longer
+        // fit their instructions' offsets, which costs a vector addition between two matrix instructions for every read.
+#pragma unroll
+        for (uint32_t& a : at) asm volatile("" : "+v"(a));
+    }
+    // Fragment i (16 lines) of c 32 kk .. 32 kk + 31 of stage S. HALF (turned): which four of the lane's eight c.
+    template <int S, int KK>
+    __device__ __forceinline__ u32x4 straight(int i) const {
+        return *(const __attribute__((address_space(3))) u32x4*)(at[KK] + S * 32768 + i * (16 * kBK * 2));
+    }
+    template <int S, int KK, int HALF>
+    __device__ __forceinline__ s16x4 turned(int i) const {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at[i] + S * 32768 + KK * 16384 + HALF * 2048));
+    }
+};
+
+template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
+__global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g) {
+    constexpr int BM = 256, BN = 256, WM = 128, WN = 128, MI = 8, NI = 8, LOADS = 16;
+    constexpr int OUT_LD = WN + 8;
+    using Pace = BigPace<P_TURNED + Q_TURNED>;
+    __shared__ __attribute__((aligned(1024))) uint16_t Ps[2][BM * kBK];
+    __shared__ __attribute__((aligned(1024))) uint16_t Qs[2][BN * kBK];
+    __shared__ __attribute__((aligned(16))) uint16_t Out_s[4][16 * OUT_LD];
+    // The groups: their first tile (and the number of all tiles behind them), first row and end.
+    __shared__ int first_tile[kBigGroups + 1], group_lo[kBigGroups], group_hi[kBigGroups];
+
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wave_m = wave / 2, wave_n = wave % 2;
+    const int l16 = lane & 15, lq = lane >> 4;
+    const int out_tiles_m = RAGGED_C ? (g.out_rows + BM - 1) / BM : 0;
+
+    if (wave == 0) {
+        int before = 0;
+        for (int base = 0; base < g.groups; base += kWave) {
+            const int e = base + lane;
+            int lo = 0, hi = 0;
+            if (e < g.groups) {
+                lo = clamp_offset(g.offsets[e], g.rows);
+                hi = clamp_offset(g.offsets[e + 1], g.rows);
+                if (hi < lo) hi = lo;
+            }
+            const int tiles = e < g.groups ? (RAGGED_C ? out_tiles_m : (hi - lo + BM - 1) / BM) * g.tiles_n : 0;
+            const int upto = before + wave_inclusive_sum(tiles, lane);
+            if (e < g.groups) {
+                first_tile[e] = upto - tiles;
+                group_lo[e] = lo;
+                group_hi[e] = hi;
+            }
+            before = __builtin_amdgcn_readlane(upto, kWave - 1);
+        }
+        if (lane == 0) first_tile[g.groups] = before;
+    }
+    __syncthreads();
+    const int all_tiles = __builtin_amdgcn_readfirstlane(first_tile[g.groups]);
+    const int grid = gridDim.x;  // a multiple of 8
+    if (static_cast<int>(blockIdx.x) >= all_tiles) return;
+
+    // One tile of the walk: what the loads and the write-back need of it, all scalar.
+    struct Tile {
+        const uint16_t *p, *q;   // first line (straight: c = 0 of it; turned: its element of row c = 0)
+        int p_lines, q_lines;    // lines that exist, at most 256 of them
+        int depth;
+        long long out;           // first element of OUT
+        int rows_left, cols_left;
+    };
+    // Tile number `id` of the walk. 256 consecutive numbers run at a time, the workgroups of XCD x being those with
+    // number % 8 == x: they take consecutive tiles, which share operand panels in that XCD's L2. Within a group eight row
+    // tiles are walked together, column tile by column tile: 32 consecutive tiles are an 8 x 4 patch.
+    auto tile_of = [&](int id) {
+        const int round0 = id / grid * grid, w = id - round0;
+        const int count = all_tiles - round0 < grid ? all_tiles - round0 : grid;
+        const int x = w % 8, per = count / 8, rem = count % 8;
+        const int tile = round0 + x * per + (x < rem ? x : rem) + w / 8;
+        int group = 0;
+        for (int base = 0; base < g.groups; base += kWave) {
+            const int e = base + lane;
+            const unsigned long long mask = __ballot(e < g.groups && first_tile[e + 1 <= g.groups ? e + 1 : g.groups] > tile);
+            if (mask) {
+                group = base + __builtin_ctzll(mask);
+                break;
+            }
+        }
+        group = __builtin_amdgcn_readfirstlane(group);
+        const int in_group = tile - __builtin_amdgcn_readfirstlane(first_tile[group]);
+        const int lo = __builtin_amdgcn_readfirstlane(group_lo[group]), hi = __builtin_amdgcn_readfirstlane(group_hi[group]);
+        const int tiles_m = RAGGED_C ? out_tiles_m : (hi - lo + BM - 1) / BM;
+        const int block = in_group / (kBigBlockM * g.tiles_n), in_block = in_group - block * kBigBlockM * g.tiles_n;
+        const int height = tiles_m - block * kBigBlockM < kBigBlockM ? tiles_m - block * kBigBlockM : kBigBlockM;
+        const int row0 = (block * kBigBlockM + in_block % height) * BM, col0 = in_block / height * BN;
+        Tile t;
+        const int rows_here = RAGGED_C ? g.out_rows : hi - lo;
+        t.rows_left = rows_here - row0;
+        t.cols_left = g.cols - col0;
+        t.p_lines = t.rows_left < BM ? t.rows_left : BM;
+        t.q_lines = t.cols_left < BN ? t.cols_left : BN;
+        if constexpr (RAGGED_C) {
+            t.depth = hi - lo;
+            t.p = g.P + lo * g.ldp + row0;
+            t.q = g.Q + lo * g.ldq + col0;
+            t.out = group * g.group_stride + row0 * g.ldo + col0;
+        } else {
+            t.depth = g.depth;
+            t.p = g.P + (lo + row0) * g.ldp;
+            t.q = g.Q + group * g.group_stride + (Q_TURNED ? static_cast<long long>(col0) : col0 * g.ldq);
+            t.out = (lo + row0) * g.ldo + col0;
+        }
+        return t;
+    };
+
+    // Load side. Straight: a wave-wide load covers 8 lines of 128 B, a pass of the four waves 32 lines; turned: 2 rows c of
+    // 512 B, a pass 8 rows. Lane offsets are the same for every tile; `odd` for the odd passes of a turned operand, whose
+    // rows have bit 3 set (see OperandTile).
+    using PT = OperandTile<BM, P_TURNED, 4>;
+    using QT = OperandTile<BN, Q_TURNED, 4>;
+    static_assert(PT::PASSES == 8 && QT::PASSES == 8, "sixteen direct loads per wave and stage");
+    const uint32_t p_ld = static_cast<uint32_t>(g.ldp) * 2u, q_ld = static_cast<uint32_t>(g.ldq) * 2u;  // bytes; below 2^22
+    const uint32_t p_off = PT::row_of(0, wave, lane) * p_ld + PT::chunk_of(0, wave, lane) * 16u;
+    const uint32_t q_off = QT::row_of(0, wave, lane) * q_ld + QT::chunk_of(0, wave, lane) * 16u;
+    const uint32_t p_odd = PT::row_of(0, wave, lane) * p_ld + PT::chunk_of(1, wave, lane) * 16u;
+    const uint32_t q_odd = QT::row_of(0, wave, lane) * q_ld + QT::chunk_of(1, wave, lane) * 16u;
+    const uint32_t p_pass = __builtin_amdgcn_readfirstlane(PT::ROWS_PER_PASS * p_ld), q_pass = __builtin_amdgcn_readfirstlane(QT::ROWS_PER_PASS * q_ld);
+    // Descriptor of stage t of a tile: straight: the lines that exist, columns from 64 t on; turned: rows 64 t on, of
+    // which the last reaches to its last line only (a chunk beyond the lines of another row is the next row's head:
+    // finite or not, it only enters lines that are not written).
+    auto descriptor_of = [&](auto turned, const uint16_t* base, int lines, int depth, uint32_t ld_bytes, int stage) {
+        constexpr bool T = decltype(turned)::value;
+        uint64_t a = reinterpret_cast<uint64_t>(base);
+        int extent;
+        if constexpr (!T) {
+            a += static_cast<uint64_t>(static_cast<uint32_t>(stage)) * (kBK * 2);
+            extent = lines * static_cast<int>(ld_bytes);
+        } else {
+            a += static_cast<uint64_t>(static_cast<uint32_t>(stage)) * (kBK * ld_bytes);
+            const int rows = scalar_max(scalar_min(depth - stage * kBK, kBK), 0);
+            extent = scalar_max((rows - 1) * static_cast<int>(ld_bytes) + lines * 2, 0);  // no rows: not above 0, as lines * 2 <= ld_bytes
+        }
+        i32x4 d;
+        d[0] = static_cast<int>(a & 0xffffffffu);
+        d[1] = static_cast<int>((a >> 32) & 0xffffu);
+        d[2] = extent;
+        d[3] = 0x00020000;
+        return d;
+    };
+    // Lane offset of a straight operand at stage t: the partial last stage ends inside a line, the padding stages beyond.
+    auto straight_offset = [&](uint32_t off, int chunk, int depth, int stage) -> uint32_t {
+        const int left = depth - stage * kBK;
+        return chunk * 8 < left ? off : kBeyondExtent;
+    };
+    const int p_chunk = PT::chunk_of(0, wave, lane), q_chunk = QT::chunk_of(0, wave, lane);
+    auto lds_of = [&](int stage, int m) -> const uint16_t* {
+        return m < 8 ? &Ps[stage][PT::lds_elem(m, wave)] : &Qs[stage][QT::lds_elem(m - 8, wave)];
+    };
+    auto aim_load = [&](int stage, int m) { set_direct_load_destination(lds_of(stage, m)); };
+    auto fire_load = [&](const i32x4& pd, const i32x4& qd, uint32_t po, uint32_t qo, uint32_t po_odd, uint32_t qo_odd, int m) {
+        if (m < 8) direct_load16_buffer_to_destination(pd, m % 2 ? po_odd : po, m * p_pass);
+        else direct_load16_buffer_to_destination(qd, m % 2 ? qo_odd : qo, (m - 8) * q_pass);
+    };
+
+    // Operand side. Fragment sets: [0] c 0..31 of the current stage; [1], [2] c 32..63 of stage 0 / stage 1.
+    BigFragments<P_TURNED> p_at;
+    BigFragments<Q_TURNED> q_at;
+    p_at.init(Ps[0], wave_m * WM, lane);
+    q_at.init(Qs[0], wave_n * WN, lane);
+    union Fragment {
+        u32x4 whole;
+        s16x4 half[2];
+    };
+    Fragment fp[3][MI], fq[3][NI];
+    f32x4 acc[MI][NI];
+    // A phase's reads in order: per fragment one (straight) or two (turned).
+    constexpr int P_READS = 8 * (1 + P_TURNED), Q_READS = 8 * (1 + Q_TURNED), SET_READS = P_READS + Q_READS;
+    auto read_one = [&](auto stage_c, auto kk_c, int set, int r) {
+        constexpr int S = decltype(stage_c)::value, KK = decltype(kk_c)::value;
+        if (r < P_READS) {
+            if constexpr (!P_TURNED) fp[set][r].whole = p_at.template straight<S, KK>(r);
+            else if (r % 2 == 0) fp[set][r / 2].half[0] = p_at.template turned<S, KK, 0>(r / 2);
+            else fp[set][r / 2].half[1] = p_at.template turned<S, KK, 1>(r / 2);
+        } else {
+            r -= P_READS;
+            if constexpr (!Q_TURNED) fq[set][r].whole = q_at.template straight<S, KK>(r);
+            else if (r % 2 == 0) fq[set][r / 2].half[0] = q_at.template turned<S, KK, 0>(r / 2);
+            else fq[set][r / 2].half[1] = q_at.template turned<S, KK, 1>(r / 2);
+        }
+    };
+    auto mfma_block = [&](int set, auto after) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int jj = 0; jj < NI; ++jj) {
+                const int j = (i & 1) ? NI - 1 - jj : jj;
+                mfma_in_place(acc[i][j], __builtin_bit_cast(bf16x8, fq[set][j].whole), __builtin_bit_cast(bf16x8, fp[set][i].whole));
+                __builtin_amdgcn_sched_barrier(0);
+                after(i * NI + jj);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    // One phase, for the stage S that holds K tile t; it fetches what `from` says at stage number `next` into S.
+    auto phase = [&](auto stage_c, const Tile& from, int next, bool wait_at_end) {
+        constexpr int S = decltype(stage_c)::value;
+        constexpr int MINE = 1 + S, OTHER = 2 - S;
+        constexpr int BARRIER_AT = Pace::kBarrierAt, GAP = Pace::kGap, READS = Pace::kReads;
+        static_assert(2 * SET_READS <= READS * BARRIER_AT && BARRIER_AT <= 64 && BARRIER_AT + (LOADS - 1) * GAP < 128, "reads and loads fit the phase");
+        const i32x4 pd = descriptor_of(std::integral_constant<bool, P_TURNED>{}, from.p, from.p_lines, from.depth, p_ld, next);
+        const i32x4 qd = descriptor_of(std::integral_constant<bool, Q_TURNED>{}, from.q, from.q_lines, from.depth, q_ld, next);
+        const uint32_t po = P_TURNED ? p_off : straight_offset(p_off, p_chunk, from.depth, next);
+        const uint32_t qo = Q_TURNED ? q_off : straight_offset(q_off, q_chunk, from.depth, next);
+        const uint32_t po_odd = P_TURNED ? p_odd : po, qo_odd = Q_TURNED ? q_odd : qo;
+        auto maybe_load = [&](int at) {
+            if (at + 1 >= BARRIER_AT && (at + 1 - BARRIER_AT) % GAP == 0 && (at + 1 - BARRIER_AT) / GAP < LOADS) aim_load(S, (at + 1 - BARRIER_AT) / GAP);
+            if (at >= BARRIER_AT && (at - BARRIER_AT) % GAP == 0 && (at - BARRIER_AT) / GAP < LOADS)
+                fire_load(pd, qd, po, qo, po_odd, qo_odd, (at - BARRIER_AT) / GAP);
+        };
+        using k0 = std::integral_constant<int, 0>;
+        using k1 = std::integral_constant<int, 1>;
+        mfma_block(OTHER, [&](int m) {
+#pragma unroll
+            for (int u = 0; u < READS; ++u) {
+                const int r = m * READS + u;
+                if (r < SET_READS) read_one(stage_c, k0{}, 0, r);
+                else if (r < 2 * SET_READS) read_one(stage_c, k1{}, MINE, r - SET_READS);
+            }
+            if (m == BARRIER_AT - 1) {
+                __builtin_amdgcn_s_waitcnt(waitcnt_imm(kVmMax, 0));
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            maybe_load(m);
+        });
+        mfma_block(0, [&](int m) { maybe_load(64 + m); });
+        if (wait_at_end) __builtin_amdgcn_s_waitcnt(waitcnt_imm(LOADS, kLgkmMax));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using s0 = std::integral_constant<int, 0>;
+    using s1 = std::integral_constant<int, 1>;
+
+    int id = blockIdx.x;
+    Tile tile = tile_of(id);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const i32x4 pd = descriptor_of(std::integral_constant<bool, P_TURNED>{}, tile.p, tile.p_lines, tile.depth, p_ld, t);
+        const i32x4 qd = descriptor_of(std::integral_constant<bool, Q_TURNED>{}, tile.q, tile.q_lines, tile.depth, q_ld, t);
+        const uint32_t po = P_TURNED ? p_off : straight_offset(p_off, p_chunk, tile.depth, t);
+        const uint32_t qo = Q_TURNED ? q_off : straight_offset(q_off, q_chunk, tile.depth, t);
+        const i32x4 pd_s = scalar_descriptor(pd), qd_s = scalar_descriptor(qd);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 4" ::: "memory");  // between a scalar register's write by the vector ALU and a load that reads it
+#pragma unroll
+        for (int m = 0; m < LOADS; ++m) {
+            aim_load(t, m);
+            asm volatile("s_nop 0" ::: "memory");  // between the write of M0 and the load
+            fire_load(pd_s, qd_s, po, qo, P_TURNED ? p_odd : po, Q_TURNED ? q_odd : qo, m);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  while (true) {  // one tile per trip, its first stages complete in LDS
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fp[2][i].whole = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < NI; ++j) fq[2][j].whole = u32x4{0u, 0u, 0u, 0u};
+    const int next_id = id + grid;
+    const bool has_next = next_id < all_tiles;
+    Tile next = tile;
+    if (has_next) next = tile_of(next_id);
+    // Stages of 64 c, an even number of at least two (those beyond the depth are zeros).
+    const int have = (tile.depth + kBK - 1) / kBK, stages = have < 2 ? 2 : have + (have & 1);
+    int t = 0;
+    do {
+        asm volatile("s_nop 4");
+        const bool last = t + 2 >= stages;
+        const int fetch = last ? (has_next ? 0 : stages - 2) : t + 2;
+        Tile from = tile;  // selected field by field, not branched on: the trips stay the same straight-line code
+        from.p = last ? next.p : tile.p;
+        from.q = last ? next.q : tile.q;
+        from.p_lines = last ? next.p_lines : tile.p_lines;
+        from.q_lines = last ? next.q_lines : tile.q_lines;
+        from.depth = last ? next.depth : tile.depth;
+        phase(s0{}, from, fetch, t != 0);  // a tile's first phase: its second stage has landed, and the last tile's stores may drain
+        phase(s1{}, from, fetch + 1, true);
+        t += 2;
+    } while (t < stages);
+    grouped_settle();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fq[2][j].whole), __builtin_bit_cast(bf16x8, fp[2][i].whole), acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));  // the next tile's first stages, before the stores queue up behind them
+    OutT* out = static_cast<OutT*>(g.OUT) + tile.out;
+    const int rows_left = tile.rows_left - wave_m * WM, cols_left = tile.cols_left - wave_n * WN;
+    out += wave_m * WM * g.ldo + wave_n * WN;
+    // 16 rows at a time through the wave's own patch of LDS, so that they leave as runs of 256 B.
+    char* mine = reinterpret_cast<char*>(Out_s[wave]);
+    constexpr int RUN = 16 / sizeof(OutT);               // values of a lane's packet
+    constexpr int SPLIT = sizeof(OutT) == 4 ? 2 : 1;     // parts of 256 B in a wave's 128 columns
+    typedef OutT OutRun __attribute__((ext_vector_type(RUN)));
+    typedef OutT OutRunAny __attribute__((ext_vector_type(RUN), aligned(sizeof(OutT))));
+    const bool whole = cols_left >= WN;
+    OutT* at = out + lq * g.ldo + RUN * l16;  // row 16 i + 4 p + lq
+    int row = lq;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+        for (int part = 0; part < SPLIT; ++part) {
+#pragma unroll
+            for (int jj = 0; jj < NI / SPLIT; ++jj) {
+                const f32x4& r = acc[i][part * (NI / SPLIT) + jj];
+                if constexpr (sizeof(OutT) == 4) *reinterpret_cast<f32x4*>(mine + l16 * (OUT_LD * 2) + jj * 64 + lq * 16) = r;
+                else *reinterpret_cast<u16x4*>(mine + l16 * (OUT_LD * 2) + jj * 32 + lq * 8) = u16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+            }
+            OutRun v[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const OutRun*>(mine + (4 * p + lq) * (OUT_LD * 2) + 16 * l16);
+            if (whole) {
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                    if (row + 4 * p < rows_left) *reinterpret_cast<OutRunAny*>(at + 4 * p * g.ldo + part * (WN / SPLIT)) = v[p];
+            } else {
+                const int left = cols_left - part * (WN / SPLIT) - RUN * l16;
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e)
+                        if (row + 4 * p < rows_left && e < left) at[4 * p * g.ldo + part * (WN / SPLIT) + e] = v[p][e];
+            }
+        }
+        at += 16 * g.ldo;
+        row += 16;
+        asm volatile("" : "+v"(at), "+v"(row));  // one address and one row number carried along, not eight of each kept
+    }
+    if (!has_next) break;
+    id = next_id;
+    tile = next;
+  }
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));  // the last, redundant loads write LDS
+}
+
+// Whether 256 x 256 tiles are worth it: enough rows a group to fill them.
+bool big_pays(const GroupedProblem& g, bool ragged_c) {
+    if (g.groups > kBigGroups || cu_count() < 8) return false;
+    if (!ragged_c) return g.rows / g.groups >= 160;
+    return g.rows / g.groups >= 128;
+}
+
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
 int run(GroupedProblem g, const char* who, hipStream_t s) {
     constexpr int BM = 128, BN = 128;
@@ -239,6 +653,11 @@ int run(GroupedProblem g, const char* who, hipStream_t s) {
     const int p_along = P_TURNED ? g.out_rows : g.depth, q_along = Q_TURNED ? g.cols : g.depth;
     const bool aligned = aligned16(g.P) && aligned16(g.Q) && g.ldp % 8 == 0 && g.ldq % 8 == 0 && (RAGGED_C || g.group_stride % 8 == 0) &&
                          p_along % 8 == 0 && q_along % 8 == 0 && g.ldp < (1 << 21) && g.ldq < (1 << 21);
+    if (aligned && big_pays(g, RAGGED_C)) {
+        g.tiles_n = ceil_div(g.cols, 256);
+        gemm_grouped_big_kernel<P_TURNED, Q_TURNED, RAGGED_C, OutT><<<dim3(static_cast<unsigned>(cu_count() / 8 * 8)), dim3(256), 0, s>>>(g);
+        return check_launch("gemm_grouped_big_kernel");
+    }
     if (aligned) gemm_grouped_kernel<BM, BN, P_TURNED, Q_TURNED, RAGGED_C, true, OutT><<<grid, dim3(256), 0, s>>>(g);
     else gemm_grouped_kernel<BM, BN, P_TURNED, Q_TURNED, RAGGED_C, false, OutT><<<grid, dim3(256), 0, s>>>(g);
     return check_launch("gemm_grouped_kernel");
