@@ -40,52 +40,49 @@ class Routing(NamedTuple):
     slots: "torch.Tensor"     # [T, k] int32: the slot of an entry, -1: none
 
 
-class _on:
-    """The device of the tensors made current, its current stream as the value: the launchers work on the current device."""
-
-    def __init__(self, name: str, first: "torch.Tensor", *others: Optional["torch.Tensor"]):
-        if not first.is_cuda:
-            raise ValueError(f"{name}: expected a tensor in device memory (cuda), got a host tensor")
-        for t in others:
-            if t is not None and t.device != first.device:
-                if not t.is_cuda:
-                    raise ValueError(f"{name}: expected a tensor in device memory (cuda), got a host tensor")
-                raise ValueError(f"{name}: tensors on different devices ({first.device}, {t.device})")
-        self.index = first.device.index
-        self.back = None
-
-    def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.index:
-            self.back = torch.cuda.current_device()
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
+def _call(function: str, name: str, tensors, *args) -> None:
+    """Calls a launcher with the current stream of the tensors' device as its last argument. The launchers work on the
+    current device, so another one is made current for the call. Kept short: with few tokens the host's time is what a
+    layer takes."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != device or device < 0:
+            if not all(t.is_cuda for t in tensors):
+                raise ValueError(f"{name}: expected a tensor in device memory (cuda), got a host tensor")
+            raise ValueError(f"{name}: tensors on different devices ({tensors[0].device}, {t.device})")
+    launch = getattr(_lib._lib or _lib.load(), function)
+    if device == torch.cuda.current_device():
+        rc = launch(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = launch(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != 0:
+        _check(rc, name)
 
 
 def _matrix(t: "torch.Tensor", dtypes, name: str, rows: Optional[int] = None, cols: Optional[int] = None) -> int:
     """Checks a row-major matrix; returns the elements between its rows."""
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: dtype {t.dtype} not in {tuple(dtypes)}")
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
-    n, m = t.shape
-    if m > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
+    n, m = shape
+    ld, one = t.stride()
+    if one != 1 and m > 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
     if n <= 1 or m == 0:
         return max(m, 1)
-    if t.stride(0) < m:
-        raise ValueError(f"{name}: rows overlap (stride {t.stride(0)}, length {m})")
-    return t.stride(0)
+    if ld < m:
+        raise ValueError(f"{name}: rows overlap (stride {ld}, length {m})")
+    return ld
 
 
 def _whole(t: "torch.Tensor", dtype, name: str, *shape: int) -> None:
     """Checks a contiguous tensor of a given shape."""
     if t.dtype != dtype:
         raise TypeError(f"{name}: dtype {t.dtype} is not {dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor")
@@ -140,9 +137,8 @@ def route_topk(logits: "torch.Tensor", k: int, renormalise: bool = True, out: Op
         out = Routing(*out)
         _whole(out.weights, torch.float32, "weights", T, k)
         _whole(out.experts, torch.int32, "experts", T, k)
-    with _on("route_topk", logits, *out) as stream:
-        _check(_lib.load().prism_route_topk(logits.data_ptr(), _TYPES[logits.dtype], ld, T, E, k, int(bool(renormalise)), out.weights.data_ptr(),
-                                            out.experts.data_ptr(), stream), "route_topk")
+    _call("prism_route_topk", "route_topk", (logits, *out), logits.data_ptr(), _TYPES[logits.dtype], ld, T, E, k, bool(renormalise), out.weights.data_ptr(),
+          out.experts.data_ptr())
     expert_plan(out.experts, E, out=out[2:])
     return out
 
@@ -162,12 +158,10 @@ def expert_plan(experts: "torch.Tensor", num_experts: int, out=None) -> Tuple["t
     _whole(offsets, torch.int32, "offsets", num_experts + 1)
     _whole(rows, torch.int32, "rows", T * k)
     _whole(slots, torch.int32, "slots", T, k)
-    lib = _lib.load()
-    with _on("expert_plan", experts, offsets, rows, slots) as stream:
-        need = lib.prism_expert_plan_workspace_bytes(T, k, num_experts)
-        workspace = torch.empty(need, dtype=torch.uint8, device=experts.device) if need > 16 else None
-        _check(lib.prism_expert_plan(experts.data_ptr(), T, k, num_experts, offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-                                     workspace.data_ptr() if workspace is not None else 0, need, stream), "expert_plan")
+    need = _lib.load().prism_expert_plan_workspace_bytes(T, k, num_experts)
+    workspace = torch.empty(need, dtype=torch.uint8, device=experts.device) if need > 16 else None
+    _call("prism_expert_plan", "expert_plan", (experts, offsets, rows, slots), experts.data_ptr(), T, k, num_experts, offsets.data_ptr(), rows.data_ptr(),
+          slots.data_ptr(), workspace.data_ptr() if workspace is not None else 0, need)
     return offsets, rows, slots
 
 
@@ -183,10 +177,8 @@ def route_topk_backward(grad_weights: "torch.Tensor", logits: "torch.Tensor", we
     _whole(experts, torch.int32, "experts", T, k)
     out = _out(out, (T, E), logits.dtype, logits)
     ldo = _matrix(out, (logits.dtype,), "out", T, E)
-    with _on("route_topk_backward", logits, grad_weights, weights, experts, out) as stream:
-        _check(_lib.load().prism_route_topk_backward(grad_weights.data_ptr(), logits.data_ptr(), _TYPES[logits.dtype], ld, weights.data_ptr(),
-                                                     experts.data_ptr(), T, E, k, int(bool(renormalise)), out.data_ptr(), ldo, stream),
-               "route_topk_backward")
+    _call("prism_route_topk_backward", "route_topk_backward", (logits, grad_weights, weights, experts, out), grad_weights.data_ptr(), logits.data_ptr(),
+          _TYPES[logits.dtype], ld, weights.data_ptr(), experts.data_ptr(), T, E, k, bool(renormalise), out.data_ptr(), ldo)
     return out
 
 
@@ -202,9 +194,8 @@ def expert_gather(x: "torch.Tensor", rows: "torch.Tensor", k: int, out: Optional
     _whole(rows, torch.int32, "rows", rows.shape[0])
     out = _out(out, (rows.shape[0], H), x.dtype, x)
     ldo = _matrix(out, (x.dtype,), "out", rows.shape[0], H)
-    with _on("expert_gather", x, rows, out) as stream:
-        _check(_lib.load().prism_expert_gather(x.data_ptr(), _TYPES[x.dtype], ldx, T, k, rows.data_ptr(), out.data_ptr(), ldo, rows.shape[0], H, stream),
-               "expert_gather")
+    _call("prism_expert_gather", "expert_gather", (x, rows, out), x.data_ptr(), _TYPES[x.dtype], ldx, T, k, rows.data_ptr(), out.data_ptr(), ldo,
+          rows.shape[0], H)
     return out
 
 
@@ -219,9 +210,8 @@ def _sum(name: str, y: "torch.Tensor", weights: Optional["torch.Tensor"], slots:
         _whole(weights, torch.float32, "weights", T, k)
     out = _out(out, (T, H), y.dtype, y)
     ldo = _matrix(out, (y.dtype,), "out", T, H)
-    with _on(name, y, weights, slots, out) as stream:
-        _check(_lib.load().prism_expert_combine(y.data_ptr(), _TYPES[y.dtype], ldy, R, weights.data_ptr() if weights is not None else 0, slots.data_ptr(),
-                                                T, k, out.data_ptr(), ldo, H, stream), name)
+    _call("prism_expert_combine", name, (y, slots, out) if weights is None else (y, weights, slots, out), y.data_ptr(), _TYPES[y.dtype], ldy, R,
+          0 if weights is None else weights.data_ptr(), slots.data_ptr(), T, k, out.data_ptr(), ldo, H)
     return out
 
 
@@ -254,9 +244,8 @@ def expert_combine_backward(grad_out: "torch.Tensor", y: "torch.Tensor", weights
     lddy = _matrix(grad_y, (y.dtype,), "grad_y", R, H)
     grad_weights = _out(grad_weights, (T, k), torch.float32, y)
     _whole(grad_weights, torch.float32, "grad_weights", T, k)
-    with _on("expert_combine_backward", y, grad_out, weights, slots, grad_y, grad_weights) as stream:
-        _check(_lib.load().prism_expert_combine_backward(grad_out.data_ptr(), _TYPES[y.dtype], ldd, y.data_ptr(), ldy, weights.data_ptr(), slots.data_ptr(),
-                                                         T, k, grad_y.data_ptr(), lddy, grad_weights.data_ptr(), R, H, stream), "expert_combine_backward")
+    _call("prism_expert_combine_backward", "expert_combine_backward", (y, grad_out, weights, slots, grad_y, grad_weights), grad_out.data_ptr(),
+          _TYPES[y.dtype], ldd, y.data_ptr(), ldy, weights.data_ptr(), slots.data_ptr(), T, k, grad_y.data_ptr(), lddy, grad_weights.data_ptr(), R, H)
     return grad_y, grad_weights
 
 
@@ -280,9 +269,8 @@ def gemm_bf16_grouped(A: "torch.Tensor", B: "torch.Tensor", offsets: "torch.Tens
     _whole(offsets, torch.int32, "offsets", G + 1)
     D = _out(D, (R, N), out_dtype, A)
     ldd = _matrix(D, _TYPES, "D", R, N)
-    with _on("gemm_bf16_grouped", A, B, offsets, D) as stream:
-        _check(_lib.load().prism_gemm_bf16_grouped(G, R, N, K, A.data_ptr(), lda, B.data_ptr(), ldb, stride, offsets.data_ptr(), D.data_ptr(), ldd,
-                                                   _TYPES[D.dtype], stream), "gemm_bf16_grouped")
+    _call("prism_gemm_bf16_grouped", "gemm_bf16_grouped", (A, B, offsets, D), G, R, N, K, A.data_ptr(), lda, B.data_ptr(), ldb, stride,
+          offsets.data_ptr(), D.data_ptr(), ldd, _TYPES[D.dtype])
     return D
 
 
@@ -296,9 +284,8 @@ def gemm_bf16_grouped_grad_a(dD: "torch.Tensor", B: "torch.Tensor", offsets: "to
     _whole(offsets, torch.int32, "offsets", G + 1)
     dA = _out(dA, (R, K), out_dtype, dD)
     lda = _matrix(dA, _TYPES, "dA", R, K)
-    with _on("gemm_bf16_grouped_grad_a", dD, B, offsets, dA) as stream:
-        _check(_lib.load().prism_gemm_bf16_grouped_grad_a(G, R, N, K, dD.data_ptr(), ldd, B.data_ptr(), ldb, stride, offsets.data_ptr(), dA.data_ptr(), lda,
-                                                          _TYPES[dA.dtype], stream), "gemm_bf16_grouped_grad_a")
+    _call("prism_gemm_bf16_grouped_grad_a", "gemm_bf16_grouped_grad_a", (dD, B, offsets, dA), G, R, N, K, dD.data_ptr(), ldd, B.data_ptr(), ldb, stride,
+          offsets.data_ptr(), dA.data_ptr(), lda, _TYPES[dA.dtype])
     return dA
 
 
@@ -318,9 +305,8 @@ def gemm_bf16_grouped_grad_b(dD: "torch.Tensor", A: "torch.Tensor", offsets: "to
     ldb, stride = _groups(dB, _TYPES, "dB", N, K)
     if dB.shape[0] != G:
         raise ValueError(f"dB: {dB.shape[0]} matrices for {G} groups")
-    with _on("gemm_bf16_grouped_grad_b", dD, A, offsets, dB) as stream:
-        _check(_lib.load().prism_gemm_bf16_grouped_grad_b(G, R, N, K, dD.data_ptr(), ldd, A.data_ptr(), lda, offsets.data_ptr(), dB.data_ptr(), ldb, stride,
-                                                          _TYPES[dB.dtype], stream), "gemm_bf16_grouped_grad_b")
+    _call("prism_gemm_bf16_grouped_grad_b", "gemm_bf16_grouped_grad_b", (dD, A, offsets, dB), G, R, N, K, dD.data_ptr(), ldd, A.data_ptr(), lda,
+          offsets.data_ptr(), dB.data_ptr(), ldb, stride, _TYPES[dB.dtype])
     return dB
 
 
@@ -358,8 +344,7 @@ def gemv_w4(x: "torch.Tensor", q: "torch.Tensor", scales: "torch.Tensor", group_
         raise ValueError(f"gemv_w4: {G} weight matrices need offsets")
     out = _out(out, (R, N), out_dtype, x)
     ldo = _matrix(out, _TYPES, "out", R, N)
-    with _on("gemv_w4", x, q, scales, zeros, offsets, out) as stream:
-        _check(_lib.load().prism_gemv_w4(G, R, N, K, x.data_ptr(), ldx, q.data_ptr(), ldq, stride, scales.data_ptr(),
-                                         zeros.data_ptr() if zeros is not None else 0, group_size, offsets.data_ptr() if offsets is not None else 0,
-                                         out.data_ptr(), ldo, _TYPES[out.dtype], stream), "gemv_w4")
+    _call("prism_gemv_w4", "gemv_w4", [t for t in (x, q, scales, zeros, offsets, out) if t is not None], G, R, N, K, x.data_ptr(), ldx, q.data_ptr(), ldq,
+          stride, scales.data_ptr(), zeros.data_ptr() if zeros is not None else 0, group_size, offsets.data_ptr() if offsets is not None else 0, out.data_ptr(),
+          ldo, _TYPES[out.dtype])
     return out
