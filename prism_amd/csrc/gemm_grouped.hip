@@ -17,14 +17,14 @@
 #include "common.h"
 #include "direct_load.h"
 #include "expert_groups.h"
+#include "few_rows.h"
+#include "tile_map.h"
 
 namespace prism {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -633,6 +633,160 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
     __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));  // the last, redundant loads write LDS
 }
 
+// ------------------------------------------------------------------------------------------- few rows: 16 a tile --
+// The forward product where a group has few rows: reading B bounds it. A wavefront takes 16 columns and a slice of K, 128 k
+// to a step; its lane reads 16 B of the column's row of B for every instruction (the four lanes of a row 64 B, the next
+// instruction's the rest of the line), so the rows need no alignment. `parts` of a column tile meet in LDS.
+constexpr int kFewWaves = 8, kFewLeast = 2, kFewStep = 128;
+
+struct FewProblem {
+    const uint16_t *A, *B;
+    const int32_t* offsets;
+    void* D;
+    long long lda, ldb, ldd, group_stride;
+    int groups, rows, N, K;
+    int tiles_n, row_tiles, k_parts, n_parts;
+};
+
+// What a wavefront works on (as W4Slice of the 4-bit weights): its lane's row of B, its complete steps first .. end - 1,
+// and whether it also has the partial last one.
+struct FewSlice {
+    const uint16_t *b, *x;
+    long long ldx;
+    int rows, first, end, K;
+    bool partial;
+};
+
+template <int ROWS>
+__device__ __forceinline__ f32x4 multiply_few(const FewSlice& p) {
+    constexpr int U = ROWS == 16 ? 1 : 2;  // steps of a round
+    constexpr int BRINGS = 16 / ROWS, I = U * 4, X_LOADS = (I + BRINGS - 1) / BRINGS;
+    const int lane = threadIdx.x % kWave, l16 = lane % 16, lq = lane / 16;
+    const uint16_t* x_row = p.x + (l16 % ROWS < p.rows ? l16 % ROWS : p.rows - 1) * p.ldx + 8 * lq;
+    const uint16_t* b_row = p.b + 8 * lq;
+    // A round: U steps of B and the x they meet, fetched two rounds ahead. Loads are waited for in order: x is not asked
+    // for later than its weights, and nothing is fetched under a condition (where two paths with different loads meet, the
+    // wait has to assume the shorter one and waits for the rounds ahead as well).
+    struct Round {
+        u32x4 b[I], x[X_LOADS];
+    };
+    auto fetch = [&](Round& r, int step) {
+#pragma unroll
+        for (int i = 0; i < I; ++i) __builtin_memcpy(&r.b[i], b_row + static_cast<long long>(step) * kFewStep + 32 * i, 16);
+#pragma unroll
+        for (int j = 0; j < X_LOADS; ++j) {
+            const int c = j * BRINGS + l16 / ROWS;  // the lane's instruction; beyond the round's, the last one's
+            __builtin_memcpy(&r.x[j], x_row + static_cast<long long>(step) * kFewStep + 32 * (c < I ? c : I - 1), 16);
+        }
+    };
+    f32x4 even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;
+    auto compute = [&](const Round& r) {
+        bf16x8 x[X_LOADS];
+#pragma unroll
+        for (int j = 0; j < X_LOADS; ++j) x[j] = __builtin_bit_cast(bf16x8, r.x[j]);
+        auto pair = [&](auto c) {
+            constexpr int C = decltype(c)::value;
+            bf16x8 a, b;
+            instruction_x<ROWS, C>(x, a);
+            instruction_x<ROWS, C + 1>(x, b);
+            even = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, r.b[C]), even, 0, 0, 0);
+            odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, __builtin_bit_cast(bf16x8, r.b[C + 1]), odd, 0, 0, 0);
+        };
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 2>{});
+        if constexpr (U == 2) {
+            pair(std::integral_constant<int, 4>{});
+            pair(std::integral_constant<int, 6>{});
+        }
+    };
+    const int rounds = p.end > p.first ? (p.end - p.first) / U : 0;
+    if (rounds > 0) {
+        auto round_at = [&](int r) { return p.first + (r < rounds ? r : rounds - 1) * U; };
+        Round a, b;
+        fetch(a, p.first);
+        fetch(b, round_at(1));
+        for (int r = 0;; r += 2) {
+            compute(a);
+            if (r + 2 >= rounds) {
+                if (r + 1 < rounds) compute(b);
+                break;
+            }
+            fetch(a, round_at(r + 2));
+            compute(b);
+            fetch(b, round_at(r + 3));
+        }
+    }
+    // What is left: complete steps that fill no round, and the partial last one, whose packets are cut at K.
+    const uint16_t* x_own = p.x + (l16 < p.rows ? l16 : p.rows - 1) * p.ldx + 8 * lq;
+    for (int step = p.first + rounds * U; step < p.end + p.partial; ++step) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = step * kFewStep + 32 * i, there = p.K - k - 8 * lq;
+            const u32x4 x = load_packet(x_own + k, there), b = load_packet(b_row + k, there);
+            even = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, b), even, 0, 0, 0);
+        }
+    }
+    return even + odd;
+}
+
+template <typename OutT>
+__global__ __launch_bounds__(kFewWaves * kWave) void gemm_grouped_few_kernel(FewProblem p) {
+    __shared__ f32x4 parts[kFewWaves * kWave];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int l16 = lane % 16, lq = lane / 16;
+    const int k_part = wave % p.k_parts, n_part = wave / p.k_parts;
+    // The row tiles of a column tile follow each other on one XCD (workgroups 8 apart), whose L2 then has its part of B.
+    const int xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds;
+    const int column = (local / p.row_tiles) * kXcds + xcd;
+    if (column >= p.tiles_n) return;
+    const GroupTile t = find_group_tile(p.offsets, p.groups, p.rows, local % p.row_tiles, 16);
+    if (t.group < 0) return;
+    const int n0 = (column * p.n_parts + n_part) * 16;
+    const int whole = p.K / kFewStep, steps = (p.K + kFewStep - 1) / kFewStep, slice = (steps + p.k_parts - 1) / p.k_parts;
+    FewSlice s;
+    s.b = p.B + t.group * p.group_stride + (n0 + l16 < p.N ? n0 + l16 : p.N - 1) * p.ldb;  // columns beyond the last repeat it
+    s.x = p.A + t.row0 * p.lda;
+    s.ldx = p.lda;
+    s.rows = t.row_end - t.row0 < 16 ? t.row_end - t.row0 : 16;
+    s.first = k_part * slice;
+    s.end = s.first + slice < whole ? s.first + slice : whole;
+    s.partial = whole < steps && s.first <= whole && whole < s.first + slice;
+    if (s.end < s.first) s.end = s.first;  // a slice beyond the last step
+    s.K = p.K;
+    f32x4 total;
+    if (s.rows == 1) total = multiply_few<1>(s);
+    else if (s.rows <= 4) total = multiply_few<4>(s);
+    else total = multiply_few<16>(s);
+    if (p.k_parts > 1) {  // the parts of a column tile, added in their order
+        parts[wave * kWave + lane] = total;
+        __syncthreads();
+        if (k_part != 0) return;
+        for (int o = 1; o < p.k_parts; ++o) total += parts[(wave + o) * kWave + lane];
+    }
+    if (n0 + l16 >= p.N) return;
+    OutT* out = static_cast<OutT*>(p.D);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+        if (4 * lq + v < s.rows) store_out(out + (t.row0 + 4 * lq + v) * p.ldd + n0 + l16, total[v]);
+}
+
+template <typename OutT>
+int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
+    FewProblem p{};
+    p.A = g.P; p.B = g.Q; p.offsets = g.offsets; p.D = g.OUT;
+    p.lda = g.ldp; p.ldb = g.ldq; p.ldd = g.ldo; p.group_stride = g.group_stride;
+    p.groups = g.groups; p.rows = g.rows; p.N = g.cols; p.K = g.depth;
+    const long long row_tiles = most_row_tiles(g.rows, g.groups, 16);
+    p.row_tiles = static_cast<int>(row_tiles);
+    p.k_parts = few_rows_k_parts(g.rows < g.groups ? g.rows : row_tiles, p.N, p.K, kFewStep, kFewWaves);
+    p.n_parts = p.k_parts < kFewLeast ? kFewLeast / p.k_parts : 1;
+    p.tiles_n = ceil_div(p.N, 16 * p.n_parts);
+    const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;
+    if (blocks > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
+    gemm_grouped_few_kernel<OutT><<<dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(p.k_parts * p.n_parts * kWave)), 0, s>>>(p);
+    return check_launch("gemm_grouped_few_kernel");
+}
+
 // Whether 256 x 256 tiles are worth it: enough rows a group to fill them.
 bool big_pays(const GroupedProblem& g, bool ragged_c) {
     if (g.groups > kBigGroups || cu_count() < 8) return false;
@@ -640,9 +794,14 @@ bool big_pays(const GroupedProblem& g, bool ragged_c) {
     return g.rows / g.groups >= 128;
 }
 
+// Whether tiles of 16 rows are worth it: a group's weights are read once per tile.
+bool few_pays(const GroupedProblem& g) { return g.rows / g.groups <= 16; }
+
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
 int run(GroupedProblem g, const char* who, hipStream_t s) {
     constexpr int BM = 128, BN = 128;
+    if constexpr (!P_TURNED && !Q_TURNED)
+        if (few_pays(g)) return run_few<OutT>(g, who, s);
     g.tiles_n = ceil_div(g.cols, BN);
     const long long tiles_m = RAGGED_C ? static_cast<long long>(g.groups) * ceil_div(g.out_rows, BM) : most_row_tiles(g.rows, g.groups, BM);
     if (tiles_m == 0) return 0;

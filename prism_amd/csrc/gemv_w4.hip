@@ -17,17 +17,15 @@
 
 #include "common.h"
 #include "expert_groups.h"
+#include "few_rows.h"
+#include "tile_map.h"
 
 namespace prism {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kW4Waves = 8, kW4Block = 128;  // wavefronts of a workgroup; k per step: 16 B of weights a lane
-constexpr int round_steps(int mt) { return mt == 4 ? 2 : 4; }  // steps fetched together, a round ahead of their use
-constexpr int kW4Lds = 60 * 1024;            // for the rows of x: two workgroups to a CU
+constexpr int kW4Waves = 8, kW4Few = 2, kW4Block = 128;  // most and fewest wavefronts of a workgroup; k per step: 16 B of weights a lane
 
 struct W4Problem {
     const uint16_t* x;
@@ -38,8 +36,8 @@ struct W4Problem {
     void* y;
     long long ldx, ldq, ldy, q_stride, s_stride;  // q_stride, s_stride: between the groups' matrices
     int groups, rows, N, K, G, n_groups;          // n_groups: scales per row
-    int tiles_n;          // workgroups along N
-    int k_parts, chunk_k; // wavefronts that share a column tile's K; k of x in LDS at a time
+    int tiles_n, row_tiles;  // workgroups along N, tiles of 16 rows
+    int k_parts, n_parts; // wavefronts that share a column tile's K, column tiles of a workgroup
 };
 
 __device__ __forceinline__ void store_y(float* p, float v) { *p = v; }
@@ -89,186 +87,225 @@ __device__ __forceinline__ u32x4 turned(u32x4 w) {
 // Scales of a step: kOne: a step is a group (G = 128); kTwo, kFour: it is two or four (64, 32); kAny: looked up.
 enum class StepScales { kOne, kTwo, kFour, kAny };
 
-// MT: tiles of 16 rows. Eight wavefronts: 8 / k_parts column tiles of 16, each by k_parts wavefronts that take every
-// k_parts-th step. The rows of x pass through LDS in chunks of chunk_k, in the order of `ordered`.
-template <StepScales SCALES, int MT, bool ZEROS, typename OutT>
-__global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Problem p) {
-    constexpr bool TURN = SCALES != StepScales::kOne;  // G below 128: an instruction's 32 k are consecutive
-    constexpr int U = round_steps(MT);
-    extern __shared__ __attribute__((aligned(16))) uint16_t xs[];
-    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int l16 = lane % 16, lq = lane / 16;
-    const int k_part = wave % p.k_parts, n_part = wave / p.k_parts;
-    const int tile = blockIdx.x / p.tiles_n, n0 = ((blockIdx.x % p.tiles_n) * (kW4Waves / p.k_parts) + n_part) * 16;
-    int row0, row_end, group = 0;
-    if (p.offsets != nullptr) {
-        const GroupTile t = find_group_tile(p.offsets, p.groups, p.rows, tile, 16 * MT);
-        if (t.group < 0) return;
-        row0 = t.row0;
-        row_end = t.row_end;
-        group = t.group;
-    } else {
-        row0 = tile * 16 * MT;
-        row_end = p.rows;
-    }
-    const int rows = row_end - row0 < 16 * MT ? row_end - row0 : 16 * MT;
-    const int n = n0 + l16 < p.N ? n0 + l16 : p.N - 1;  // columns beyond the last repeat it and are not written
-    const uint8_t* q = p.q + group * p.q_stride + n * p.ldq;
-    const uint16_t* scales = p.scales + group * p.s_stride + static_cast<long long>(n) * p.n_groups;
-    const uint8_t* zeros = ZEROS ? p.zeros + group * p.s_stride + static_cast<long long>(n) * p.n_groups : nullptr;
+constexpr int parts_of(StepScales s) { return s == StepScales::kOne ? 1 : (s == StepScales::kTwo ? 2 : 4); }
 
-    // A round: the weights, scales and zero points of U steps, fetched a round ahead.
-    constexpr int PARTS = SCALES == StepScales::kOne ? 1 : (SCALES == StepScales::kTwo ? 2 : 4);
+// What a wavefront works on: its lane's row of weights and scales, its steps (first .. first + slice - 1 of `steps`, of
+// which `whole` are complete), and the tile's rows of x.
+struct W4Slice {
+    const uint8_t* q;
+    const uint16_t* scales;
+    const uint8_t* zeros;
+    const uint16_t* x;
+    long long ldx;
+    int rows, first, slice, whole, steps, K, G;
+};
+
+// The 16 x 16 result of a slice, 4 rows and a column to a lane, for up to ROWS rows of x (1, 4 or 16; see instruction_x).
+template <StepScales SCALES, bool ZEROS, int ROWS>
+__device__ __forceinline__ f32x4 multiply_slice(const W4Slice& p) {
+    constexpr bool TURN = SCALES != StepScales::kOne;  // G below 128: an instruction's 32 k are consecutive
+    constexpr int PARTS = parts_of(SCALES), PER = 4 / PARTS;  // parts of a step with a scale each, instructions of a part
+    constexpr int U = ROWS == 16 ? 2 : 4;                     // steps of a round
+    constexpr int BRINGS = 16 / ROWS, X_LOADS = U * 4 / BRINGS;
+    const int lane = threadIdx.x % kWave, l16 = lane % 16, lq = lane / 16;
+    const uint16_t* x_row = p.x + (l16 % ROWS < p.rows ? l16 % ROWS : p.rows - 1) * p.ldx + (TURN ? 8 : 32) * lq;
+    // A round: the weights, scales and zero points of U steps and the x they meet, fetched two rounds ahead. Loads are
+    // waited for in order: x is not asked for later than its weights, and nothing is fetched under a condition (where two
+    // paths with different loads meet, the wait has to assume the shorter one and waits for the rounds ahead as well).
     struct Round {
-        u32x4 w[U];
-        uint16_t s[U][PARTS];
-        uint8_t z[U][PARTS];
+        u32x4 w[U], x[X_LOADS];
+        uint16_t s[U * PARTS];
+        uint8_t z[U * PARTS];
     };
-    const int whole = p.K / kW4Block, steps = (p.K + kW4Block - 1) / kW4Block;
-    auto fetch = [&](Round& r, int round) {
-        if (whole == 0) return;
+    // FULL: all U steps from `first` on are complete ones; else those that are not fetch the last complete one again.
+    auto fetch = [&](auto full, Round& r, int first) {
+        constexpr bool FULL = decltype(full)::value;
+        auto step_of = [&](int u) { return FULL || first + u < p.whole ? first + u : p.whole - 1; };
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = k_part + (round * U + u) * p.k_parts, step = at < whole ? at : whole - 1;
-            __builtin_memcpy(&r.w[u], q + static_cast<long long>(step) * (kW4Block / 2) + lq * 16, 16);
-            if constexpr (SCALES != StepScales::kAny) {
-                __builtin_memcpy(r.s[u], scales + step * PARTS, PARTS * 2);
-                if constexpr (ZEROS) __builtin_memcpy(r.z[u], zeros + step * PARTS, PARTS);
-            } else {
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&r.w[u], p.q + static_cast<long long>(step_of(u)) * (kW4Block / 2), 16);
+#pragma unroll
+        for (int j = 0; j < X_LOADS; ++j) {
+            const int c = j * BRINGS + l16 / ROWS;  // the lane's instruction of the round
+            __builtin_memcpy(&r.x[j], x_row + step_of(c / 4) * kW4Block + (TURN ? 32 : 8) * (c % 4), 16);
+        }
+        if constexpr (FULL && SCALES != StepScales::kAny) {
+            __builtin_memcpy(r.s, p.scales + first * PARTS, U * PARTS * 2);
+            if constexpr (ZEROS) __builtin_memcpy(r.z, p.zeros + first * PARTS, U * PARTS);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < PARTS; ++i) {
-                    const int gi = (step * kW4Block + i * 32) / p.G;
-                    r.s[u][i] = scales[gi];
-                    if constexpr (ZEROS) r.z[u][i] = zeros[gi];
+                    const int gi = SCALES != StepScales::kAny ? step_of(u) * PARTS + i : (step_of(u) * kW4Block + i * 32) / p.G;
+                    r.s[u * PARTS + i] = p.scales[gi];
+                    if constexpr (ZEROS) r.z[u * PARTS + i] = p.zeros[gi];
                 }
-            }
         }
     };
-    f32x4 total[MT] = {};
+    f32x4 total = {0.0f, 0.0f, 0.0f, 0.0f};
     const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
     const bf16x8 ones = __builtin_bit_cast(bf16x8, one);
-    const int stride = p.chunk_k + 8;  // of a row in LDS: padded by one packet
-    const uint16_t* x_lane[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) x_lane[m] = xs + (m * 16 + l16 < rows ? m * 16 + l16 : rows - 1) * stride + (TURN ? 8 : 32) * lq;
-    // The instructions of one step, whose first k is at element `at` of the chunk.
-    auto step = [&](u32x4 w, const uint16_t (&s)[PARTS], const uint8_t (&z)[PARTS], int at) {
+    auto multiply = [&](u32x4 w, const bf16x8 (&x)[4], const uint16_t* s, const uint8_t* z) {
         if constexpr (TURN) w = turned(w);
-        f32x4 dot[MT], sum[MT];
+        f32x4 dot[PARTS], sum[PARTS];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            constexpr int PER = 4 / PARTS;
-            const bf16x8 wv = weights_of(w[i]);
+            if (i % PER == 0) dot[i / PER] = sum[i / PER] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            dot[i / PER] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], weights_of(w[i]), dot[i / PER], 0, 0, 0);
+            sum[i / PER] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], ones, sum[i / PER], 0, 0, 0);
+        }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (i % PER == 0) dot[m] = sum[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                const bf16x8 a = *reinterpret_cast<const bf16x8*>(x_lane[m] + at + (TURN ? 32 : 8) * i);
-                dot[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, wv, dot[m], 0, 0, 0);
-                sum[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ones, sum[m], 0, 0, 0);
-            }
-            if (i % PER == PER - 1) {
-                const float scale = __builtin_bit_cast(float, static_cast<uint32_t>(s[i / PER]) << 16), zero = ZEROS ? 16.0f + z[i / PER] : 24.0f;
+        for (int part = 0; part < PARTS; ++part) {
+            const float scale = __builtin_bit_cast(float, static_cast<uint32_t>(s[part]) << 16), zero = ZEROS ? 16.0f + z[part] : 24.0f;
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) total[m][v] = __builtin_fmaf(scale, __builtin_fmaf(-zero, sum[m][v], dot[m][v]), total[m][v]);
-            }
+            for (int v = 0; v < (ROWS == 1 ? 1 : 4); ++v) total[v] = __builtin_fmaf(scale, __builtin_fmaf(-zero, sum[part][v], dot[part][v]), total[v]);
         }
     };
-    // Chunk of x from k = first on, zeros beyond K.
-    auto stage = [&](int first) {
-        const int left = (steps * kW4Block - first) / 8, packets = left < p.chunk_k / 8 ? left : p.chunk_k / 8;
-        for (int i = threadIdx.x; i < rows * packets; i += kW4Waves * kWave) {
-            const int row = i / packets, c = (i - row * packets) * 8, k = first + c;
-            const uint16_t* x = p.x + (row0 + row) * p.ldx + k;
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (k + 8 <= p.K) {
-                __builtin_memcpy(&v, x, 16);
-            } else {
+    auto compute = [&](const Round& r, int count) {
+        bf16x8 x[X_LOADS];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k + e < p.K) v[e / 2] |= static_cast<uint32_t>(x[e]) << (16 * (e % 2));
-            }
-            *reinterpret_cast<bf16x8*>(xs + row * stride + c) = ordered(v);
+        for (int j = 0; j < X_LOADS; ++j) x[j] = ordered(r.x[j]);
+        auto step = [&](auto u_c) {
+            constexpr int u = decltype(u_c)::value;
+            if (u >= count) return;
+            bf16x8 mine[4];
+            instruction_x<ROWS, u * 4 + 0>(x, mine[0]);
+            instruction_x<ROWS, u * 4 + 1>(x, mine[1]);
+            instruction_x<ROWS, u * 4 + 2>(x, mine[2]);
+            instruction_x<ROWS, u * 4 + 3>(x, mine[3]);
+            multiply(r.w[u], mine, &r.s[u * PARTS], &r.z[u * PARTS]);
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        if constexpr (U == 4) {
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
         }
     };
-    const int per_round = p.k_parts * U, rounds = (steps + per_round - 1) / per_round, per_chunk = p.chunk_k / (per_round * kW4Block);
-    Round now, ahead;
-    fetch(now, 0);
-    for (int r = 0; r < rounds; ++r) {
-        const int chunk0 = r / per_chunk * per_chunk * per_round;  // the chunk's first step
-        if (r % per_chunk == 0) {
-            if (r > 0) __syncthreads();
-            stage(chunk0 * kW4Block);
-            __syncthreads();
+    using yes = std::integral_constant<bool, true>;
+    using no = std::integral_constant<bool, false>;
+    const int end = p.first + p.slice < p.whole ? p.first + p.slice : p.whole, rounds = end > p.first ? (end - p.first) / U : 0;
+    if (rounds > 0) {
+        auto round_at = [&](int r) { return p.first + (r < rounds ? r : rounds - 1) * U; };
+        Round a, b;
+        fetch(yes{}, a, p.first);
+        fetch(yes{}, b, round_at(1));
+        for (int r = 0;; r += 2) {
+            compute(a, U);
+            if (r + 2 >= rounds) {
+                if (r + 1 < rounds) compute(b, U);
+                break;
+            }
+            fetch(yes{}, a, round_at(r + 2));
+            compute(b, U);
+            fetch(yes{}, b, round_at(r + 3));
         }
-        if (r + 1 < rounds) fetch(ahead, r + 1);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = k_part + (r * U + u) * p.k_parts;
-            if (at < whole) step(now.w[u], now.s[u], now.z[u], (at - chunk0) * kW4Block);
-        }
-        now = ahead;
     }
-    if (whole < steps && whole % p.k_parts == k_part) {  // the partial last step: nothing is read beyond the row
-        const int chunk0 = (rounds - 1) / per_chunk * per_chunk * per_round, bytes = (p.K + 1) / 2;
+    const int behind = p.first + rounds * U;
+    if (behind < end) {  // fewer than U complete steps are left
+        Round a;
+        fetch(no{}, a, behind);
+        compute(a, end - behind);
+    }
+    if (p.whole < p.steps && p.first <= p.whole && p.whole < p.first + p.slice) {  // the partial last step: nothing is read beyond the rows
+        const int bytes = (p.K + 1) / 2 - p.whole * (kW4Block / 2) - lq * 16;
         u32x4 w = {0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int b = 0; b < 16; ++b) {
-            const int at = whole * (kW4Block / 2) + lq * 16 + b;
-            if (at < bytes) w[b / 4] |= static_cast<uint32_t>(q[at]) << (8 * (b % 4));
+        for (int i = 0; i < 16; ++i)
+            if (i < bytes) w[i / 4] |= static_cast<uint32_t>(p.q[static_cast<long long>(p.whole) * (kW4Block / 2) + i]) << (8 * (i % 4));
+        bf16x8 x[4];
+        const uint16_t* own = p.x + (l16 < p.rows ? l16 : p.rows - 1) * p.ldx + p.whole * kW4Block + (TURN ? 8 : 32) * lq;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int left = p.K - p.whole * kW4Block - (TURN ? 8 : 32) * lq - (TURN ? 32 : 8) * i;
+            u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) v[e / 2] |= static_cast<uint32_t>(own[(TURN ? 32 : 8) * i + e]) << (16 * (e % 2));
+            x[i] = ordered(v);
         }
         uint16_t s[PARTS];
         uint8_t z[PARTS];
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-            const int k = whole * kW4Block + i * (kW4Block / PARTS), gi = (k < p.K ? k : p.K - 1) / p.G;
-            s[i] = scales[gi];
-            z[i] = ZEROS ? zeros[gi] : 0;
+            const int k = p.whole * kW4Block + i * (kW4Block / PARTS), gi = (k < p.K ? k : p.K - 1) / p.G;
+            s[i] = p.scales[gi];
+            z[i] = ZEROS ? p.zeros[gi] : 0;
         }
-        step(w, s, z, (whole - chunk0) * kW4Block);
+        multiply(w, x, s, z);
     }
+    return total;
+}
+
+// Eight wavefronts for up to 16 rows: 8 / k_parts column tiles of 16, each by k_parts wavefronts that take consecutive
+// steps (a slice each).
+template <StepScales SCALES, bool ZEROS, typename OutT>
+__global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Problem p) {
+    __shared__ f32x4 parts[kW4Waves * kWave];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int l16 = lane % 16, lq = lane / 16;
+    const int k_part = wave % p.k_parts, n_part = wave / p.k_parts;
+    // Workgroups 8 apart run on one XCD: the row tiles of a column tile follow each other there, so that its L2 has the
+    // weights when the second one asks for them.
+    const int xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds;
+    const int tile = local % p.row_tiles, column = (local / p.row_tiles) * kXcds + xcd;
+    if (column >= p.tiles_n) return;
+    const int n0 = (column * p.n_parts + n_part) * 16;
+    int row0, row_end, group = 0;
+    if (p.offsets != nullptr) {
+        const GroupTile t = find_group_tile(p.offsets, p.groups, p.rows, tile, 16);
+        if (t.group < 0) return;
+        row0 = t.row0;
+        row_end = t.row_end;
+        group = t.group;
+    } else {
+        row0 = tile * 16;
+        row_end = p.rows;
+    }
+    const int n = n0 + l16 < p.N ? n0 + l16 : p.N - 1;  // columns beyond the last repeat it and are not written
+    const long long scale_row = group * p.s_stride + static_cast<long long>(n) * p.n_groups;
+    W4Slice s;
+    s.q = p.q + group * p.q_stride + n * p.ldq + lq * 16;
+    s.scales = p.scales + scale_row;
+    s.zeros = ZEROS ? p.zeros + scale_row : nullptr;
+    s.x = p.x + row0 * p.ldx;
+    s.ldx = p.ldx;
+    s.rows = row_end - row0 < 16 ? row_end - row0 : 16;
+    s.whole = p.K / kW4Block;
+    s.steps = (p.K + kW4Block - 1) / kW4Block;
+    s.slice = (s.steps + p.k_parts - 1) / p.k_parts;
+    s.first = k_part * s.slice;
+    s.K = p.K;
+    s.G = p.G;
+    f32x4 total;
+    if (s.rows == 1) total = multiply_slice<SCALES, ZEROS, 1>(s);
+    else if (s.rows <= 4) total = multiply_slice<SCALES, ZEROS, 4>(s);
+    else total = multiply_slice<SCALES, ZEROS, 16>(s);
     // The parts of a column tile, added in their order.
-    f32x4* part = reinterpret_cast<f32x4*>(xs);  // [wave][MT][64]
     if (p.k_parts > 1) {
-        __syncthreads();
-#pragma unroll
-        for (int m = 0; m < MT; ++m) part[(wave * MT + m) * kWave + lane] = total[m];
+        parts[wave * kWave + lane] = total;
         __syncthreads();
         if (k_part != 0) return;
-        for (int o = 1; o < p.k_parts; ++o)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) total[m] += part[((wave + o) * MT + m) * kWave + lane];
+        for (int o = 1; o < p.k_parts; ++o) total += parts[(wave + o) * kWave + lane];
     }
     if (n0 + l16 >= p.N) return;
     OutT* y = static_cast<OutT*>(p.y);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int row = m * 16 + 4 * lq + v;
-            if (row < rows) store_y(y + (row0 + row) * p.ldy + n0 + l16, total[m][v]);
-        }
-}
-
-template <StepScales SCALES, int MT>
-int go(const W4Problem& p, int out_type, dim3 grid, size_t lds, hipStream_t s) {
-    const dim3 block(kW4Waves * kWave);
-    if (p.zeros != nullptr) {
-        if (out_type == kTypeF32) gemv_w4_kernel<SCALES, MT, true, float><<<grid, block, lds, s>>>(p);
-        else gemv_w4_kernel<SCALES, MT, true, uint16_t><<<grid, block, lds, s>>>(p);
-    } else {
-        if (out_type == kTypeF32) gemv_w4_kernel<SCALES, MT, false, float><<<grid, block, lds, s>>>(p);
-        else gemv_w4_kernel<SCALES, MT, false, uint16_t><<<grid, block, lds, s>>>(p);
-    }
-    return check_launch("gemv_w4_kernel");
+    for (int v = 0; v < 4; ++v)
+        if (4 * lq + v < s.rows) store_y(y + (row0 + 4 * lq + v) * p.ldy + n0 + l16, total[v]);
 }
 
 template <StepScales SCALES>
-int go_tiles(const W4Problem& p, int mt, int out_type, dim3 grid, size_t lds, hipStream_t s) {
-    if (mt == 1) return go<SCALES, 1>(p, out_type, grid, lds, s);
-    if (mt == 2) return go<SCALES, 2>(p, out_type, grid, lds, s);
-    return go<SCALES, 4>(p, out_type, grid, lds, s);
+int go(const W4Problem& p, int out_type, dim3 grid, hipStream_t s) {
+    const dim3 block(static_cast<unsigned>(p.k_parts * p.n_parts * kWave));
+    if (p.zeros != nullptr) {
+        if (out_type == kTypeF32) gemv_w4_kernel<SCALES, true, float><<<grid, block, 0, s>>>(p);
+        else gemv_w4_kernel<SCALES, true, uint16_t><<<grid, block, 0, s>>>(p);
+    } else {
+        if (out_type == kTypeF32) gemv_w4_kernel<SCALES, false, float><<<grid, block, 0, s>>>(p);
+        else gemv_w4_kernel<SCALES, false, uint16_t><<<grid, block, 0, s>>>(p);
+    }
+    return check_launch("gemv_w4_kernel");
 }
 
 }  // namespace
@@ -302,29 +339,20 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
         meets(scales, static_cast<uintptr_t>(groups) * p.s_stride * 2) || meets(zeros, static_cast<uintptr_t>(groups) * p.s_stride) ||
         meets(offsets, (static_cast<uintptr_t>(groups) + 1) * 4))
         return fail(1, "%s: the output overlaps an input", who);
-    // Rows a tile: 16 cost what one costs; more are worth it when a group fills them, since every tile reads the group's
-    // weights again.
-    const long long per_group = ceil_div(rows, static_cast<long long>(groups));
-    const int mt = per_group <= 16 ? 1 : (per_group <= 32 ? 2 : 4);
-    const long long tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16 * mt) : ceil_div(rows, static_cast<long long>(16 * mt));
-    // Rows of x in LDS at a time: a chunk is a whole number of rounds, so many wavefronts to a column tile need few rows.
-    const int most_rows = offsets == nullptr && rows < 16 * mt ? static_cast<int>(rows) : (rows < 16 * mt ? static_cast<int>(rows) : 16 * mt);
-    const int fits = kW4Lds / (2 * most_rows) - 8;
-    p.k_parts = kW4Waves;
-    const int part_k = round_steps(mt) * kW4Block;  // of a wavefront's round
-    while (p.k_parts > 1 && (p.k_parts * part_k > fits || p.k_parts * part_k / 2 >= K)) p.k_parts /= 2;
-    const int round_k = p.k_parts * part_k;
-    const int wanted = ceil_div(K > 0 ? K : 1, round_k);
-    p.chunk_k = round_k * (fits / round_k < wanted ? fits / round_k : wanted);
-    const size_t x_bytes = static_cast<size_t>(most_rows) * (p.chunk_k + 8) * 2, part_bytes = static_cast<size_t>(kW4Waves) * mt * kWave * 16;
-    const size_t lds = x_bytes > part_bytes ? x_bytes : part_bytes;
-    p.tiles_n = ceil_div(N, 16 * (kW4Waves / p.k_parts));
-    if (tiles * p.tiles_n > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
-    const dim3 grid(static_cast<unsigned>(tiles * p.tiles_n));
-    if (group_size == 128) return go_tiles<StepScales::kOne>(p, mt, out_type, grid, lds, s);
-    if (group_size == 64) return go_tiles<StepScales::kTwo>(p, mt, out_type, grid, lds, s);
-    if (group_size == 32) return go_tiles<StepScales::kFour>(p, mt, out_type, grid, lds, s);
-    return go_tiles<StepScales::kAny>(p, mt, out_type, grid, lds, s);
+    const long long row_tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16) : ceil_div(rows, 16ll);
+    // Of a group table's tiles about as many exist as there are rows or groups.
+    const long long busy = offsets != nullptr ? (rows < groups ? rows : row_tiles) : row_tiles;
+    p.k_parts = few_rows_k_parts(busy, N, K, kW4Block, kW4Waves);
+    p.n_parts = p.k_parts < kW4Few ? kW4Few / p.k_parts : 1;
+    p.tiles_n = ceil_div(N, 16 * p.n_parts);
+    const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;
+    if (blocks > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
+    p.row_tiles = static_cast<int>(row_tiles);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (group_size == 128) return go<StepScales::kOne>(p, out_type, grid, s);
+    if (group_size == 64) return go<StepScales::kTwo>(p, out_type, grid, s);
+    if (group_size == 32) return go<StepScales::kFour>(p, out_type, grid, s);
+    return go<StepScales::kAny>(p, out_type, grid, s);
 }
 
 }  // namespace prism
