@@ -29,9 +29,9 @@ __device__ __forceinline__ void instruction_x(const bf16x8 (&x)[LOADS], bf16x8& 
 
 // How a column tile's K is shared: by as few wavefronts as give every CU eight of them (each has a fixed cost, and their
 // parts meet at the end), not more than there are steps of step_k. `busy`: the row tiles that exist, about.
-inline int few_rows_k_parts(long long busy, int N, int K, int step_k, int most) {
+inline int few_rows_k_parts(long long busy, int N, int K, int step_k, int most, int per_cu) {
     int parts = 1;
-    while (parts < most && busy * ceil_div(N, 16) * parts < 8ll * cu_count() && parts * step_k < K) parts *= 2;
+    while (parts < most && busy * ceil_div(N, 16) * parts < static_cast<long long>(per_cu) * cu_count() && parts * step_k < K) parts *= 2;
     return parts;
 }
 

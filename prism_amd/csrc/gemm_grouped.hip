@@ -258,7 +258,8 @@ __device__ __forceinline__ int scalar_max(int a, int b) {
 }
 
 constexpr int kBigGroups = 1024;  // groups that the table in LDS holds
-constexpr int kBigBlockM = 8;     // row tiles of a group that are walked together (see tile order below)
+constexpr int kBigBlockM = 8;     // row tiles of a group that are walked together (see list_tiles)
+constexpr int kList = 32;         // tiles of a workgroup that are worked out together
 
 // Behind how many of a phase's 128 matrix instructions the barrier that frees the stage sits, and the instructions
 // between two loads.
@@ -308,6 +309,8 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
     __shared__ __attribute__((aligned(16))) uint16_t Out_s[4][16 * OUT_LD];
     // The groups: their first tile (and the number of all tiles behind them), first row and end.
     __shared__ int first_tile[kBigGroups + 1], group_lo[kBigGroups], group_hi[kBigGroups];
+    __shared__ long long list_at[kList][3];
+    __shared__ int list_left[kList][3];
 
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -349,47 +352,58 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
         long long out;           // first element of OUT
         int rows_left, cols_left;
     };
-    // Tile number `id` of the walk. 256 consecutive numbers run at a time, the workgroups of XCD x being those with
-    // number % 8 == x: they take consecutive tiles, which share operand panels in that XCD's L2. Within a group eight row
-    // tiles are walked together, column tile by column tile: 32 consecutive tiles are an 8 x 4 patch.
-    auto tile_of = [&](int id) {
+    // The workgroup's next tiles, kList at a time: a lane of the first wavefront works one out (some 200 instructions and a
+    // dozen dependent LDS reads, 2 us if every tile did it for itself at its head).
+    // 256 consecutive numbers of the walk run at a time, the workgroups of XCD x being those with number % 8 == x: they take
+    // consecutive tiles, which share operand panels in that XCD's L2. Within a group eight row tiles are walked together,
+    // column tile by column tile: 32 consecutive tiles are an 8 x 4 patch.
+    auto list_tiles = [&](int first_id) {
+        const int id = first_id + lane * grid;
+        if (lane >= kList || id >= all_tiles) return;
         const int round0 = id / grid * grid, w = id - round0;
         const int count = all_tiles - round0 < grid ? all_tiles - round0 : grid;
         const int x = w % 8, per = count / 8, rem = count % 8;
         const int tile = round0 + x * per + (x < rem ? x : rem) + w / 8;
-        int group = 0;
-        for (int base = 0; base < g.groups; base += kWave) {
-            const int e = base + lane;
-            const unsigned long long mask = __ballot(e < g.groups && first_tile[e + 1 <= g.groups ? e + 1 : g.groups] > tile);
-            if (mask) {
-                group = base + __builtin_ctzll(mask);
-                break;
-            }
-        }
-        group = __builtin_amdgcn_readfirstlane(group);
-        const int in_group = tile - __builtin_amdgcn_readfirstlane(first_tile[group]);
-        const int lo = __builtin_amdgcn_readfirstlane(group_lo[group]), hi = __builtin_amdgcn_readfirstlane(group_hi[group]);
+        int group = 0;  // the last one whose first tile is not behind this one
+        for (int step = kBigGroups / 2; step > 0; step /= 2)
+            if (group + step < g.groups && first_tile[group + step] <= tile) group += step;
+        const int in_group = tile - first_tile[group], lo = group_lo[group], hi = group_hi[group];
         const int tiles_m = RAGGED_C ? out_tiles_m : (hi - lo + BM - 1) / BM;
         const int block = in_group / (kBigBlockM * g.tiles_n), in_block = in_group - block * kBigBlockM * g.tiles_n;
         const int height = tiles_m - block * kBigBlockM < kBigBlockM ? tiles_m - block * kBigBlockM : kBigBlockM;
         const int row0 = (block * kBigBlockM + in_block % height) * BM, col0 = in_block / height * BN;
+        long long p, q, out;
+        if constexpr (RAGGED_C) {
+            p = lo * g.ldp + row0;
+            q = lo * g.ldq + col0;
+            out = group * g.group_stride + row0 * g.ldo + col0;
+        } else {
+            p = (lo + row0) * g.ldp;
+            q = group * g.group_stride + (Q_TURNED ? static_cast<long long>(col0) : col0 * g.ldq);
+            out = (lo + row0) * g.ldo + col0;
+        }
+        list_at[lane][0] = p;
+        list_at[lane][1] = q;
+        list_at[lane][2] = out;
+        list_left[lane][0] = (RAGGED_C ? g.out_rows : hi - lo) - row0;
+        list_left[lane][1] = g.cols - col0;
+        list_left[lane][2] = RAGGED_C ? hi - lo : g.depth;
+    };
+    auto listed_tile = [&](int i) {
+        auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        auto scalar64 = [&](long long v) {
+            return static_cast<long long>((static_cast<unsigned long long>(static_cast<uint32_t>(scalar(static_cast<int>(v >> 32)))) << 32) |
+                                          static_cast<uint32_t>(scalar(static_cast<int>(v & 0xffffffffll))));
+        };
         Tile t;
-        const int rows_here = RAGGED_C ? g.out_rows : hi - lo;
-        t.rows_left = rows_here - row0;
-        t.cols_left = g.cols - col0;
+        t.p = g.P + scalar64(list_at[i][0]);
+        t.q = g.Q + scalar64(list_at[i][1]);
+        t.out = scalar64(list_at[i][2]);
+        t.rows_left = scalar(list_left[i][0]);
+        t.cols_left = scalar(list_left[i][1]);
+        t.depth = scalar(list_left[i][2]);
         t.p_lines = t.rows_left < BM ? t.rows_left : BM;
         t.q_lines = t.cols_left < BN ? t.cols_left : BN;
-        if constexpr (RAGGED_C) {
-            t.depth = hi - lo;
-            t.p = g.P + lo * g.ldp + row0;
-            t.q = g.Q + lo * g.ldq + col0;
-            t.out = group * g.group_stride + row0 * g.ldo + col0;
-        } else {
-            t.depth = g.depth;
-            t.p = g.P + (lo + row0) * g.ldp;
-            t.q = g.Q + group * g.group_stride + (Q_TURNED ? static_cast<long long>(col0) : col0 * g.ldq);
-            t.out = (lo + row0) * g.ldo + col0;
-        }
         return t;
     };
 
@@ -521,8 +535,10 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
     using s0 = std::integral_constant<int, 0>;
     using s1 = std::integral_constant<int, 1>;
 
-    int id = blockIdx.x;
-    Tile tile = tile_of(id);
+    int id = blockIdx.x, at = 0;  // the current tile and its place in the list
+    if (wave == 0) list_tiles(id);
+    __syncthreads();
+    Tile tile = listed_tile(0);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const i32x4 pd = descriptor_of(std::integral_constant<bool, P_TURNED>{}, tile.p, tile.p_lines, tile.depth, p_ld, t);
@@ -555,7 +571,15 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
     const int next_id = id + grid;
     const bool has_next = next_id < all_tiles;
     Tile next = tile;
-    if (has_next) next = tile_of(next_id);
+    if (has_next) {
+        if (++at == kList) {
+            at = 0;
+            lds_barrier();  // every wavefront has its copy of the last tile of the list
+            if (wave == 0) list_tiles(next_id);
+            lds_barrier();
+        }
+        next = listed_tile(at);
+    }
     // Stages of 64 c, an even number of at least two (those beyond the depth are zeros).
     const int have = (tile.depth + kBK - 1) / kBK, stages = have < 2 ? 2 : have + (have & 1);
     int t = 0;
@@ -593,39 +617,49 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
     constexpr int SPLIT = sizeof(OutT) == 4 ? 2 : 1;     // parts of 256 B in a wave's 128 columns
     typedef OutT OutRun __attribute__((ext_vector_type(RUN)));
     typedef OutT OutRunAny __attribute__((ext_vector_type(RUN), aligned(sizeof(OutT))));
-    const bool whole = cols_left >= WN;
-    OutT* at = out + lq * g.ldo + RUN * l16;  // row 16 i + 4 p + lq
+    OutT* to = out + lq * g.ldo + RUN * l16;  // row 16 i + 4 p + lq
     int row = lq;
+    const long long row4 = 4 * g.ldo;
+    auto write_rows = [&](auto inside) {  // inside: the wave's 128 x 128 lie inside OUT
+        constexpr bool INSIDE = decltype(inside)::value;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
+        for (int i = 0; i < MI; ++i) {
 #pragma unroll
-        for (int part = 0; part < SPLIT; ++part) {
+            for (int part = 0; part < SPLIT; ++part) {
 #pragma unroll
-            for (int jj = 0; jj < NI / SPLIT; ++jj) {
-                const f32x4& r = acc[i][part * (NI / SPLIT) + jj];
-                if constexpr (sizeof(OutT) == 4) *reinterpret_cast<f32x4*>(mine + l16 * (OUT_LD * 2) + jj * 64 + lq * 16) = r;
-                else *reinterpret_cast<u16x4*>(mine + l16 * (OUT_LD * 2) + jj * 32 + lq * 8) = u16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+                for (int jj = 0; jj < NI / SPLIT; ++jj) {
+                    asm volatile("" : "+a"(acc[i][part * (NI / SPLIT) + jj]));  // conversions stay here: moved in front of the branch they spill
+                    const f32x4& r = acc[i][part * (NI / SPLIT) + jj];
+                    if constexpr (sizeof(OutT) == 4) *reinterpret_cast<f32x4*>(mine + l16 * (OUT_LD * 2) + jj * 64 + lq * 16) = r;
+                    else *reinterpret_cast<u16x4*>(mine + l16 * (OUT_LD * 2) + jj * 32 + lq * 8) = u16x4{to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+                }
+                OutRun v[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const OutRun*>(mine + (4 * p + lq) * (OUT_LD * 2) + 16 * l16);
+                OutT* at = to + part * (WN / SPLIT);
+                if constexpr (INSIDE) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) *reinterpret_cast<OutRunAny*>(at + p * row4) = v[p];
+                } else {
+                    const int left = cols_left - part * (WN / SPLIT) - RUN * l16;
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        if (row + 4 * p >= rows_left) continue;
+                        if (left >= RUN) *reinterpret_cast<OutRunAny*>(at + p * row4) = v[p];
+                        else
+#pragma unroll
+                            for (int e = 0; e < RUN; ++e)
+                                if (e < left) at[p * row4 + e] = v[p][e];
+                    }
+                }
             }
-            OutRun v[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const OutRun*>(mine + (4 * p + lq) * (OUT_LD * 2) + 16 * l16);
-            if (whole) {
-#pragma unroll
-                for (int p = 0; p < 4; ++p)
-                    if (row + 4 * p < rows_left) *reinterpret_cast<OutRunAny*>(at + 4 * p * g.ldo + part * (WN / SPLIT)) = v[p];
-            } else {
-                const int left = cols_left - part * (WN / SPLIT) - RUN * l16;
-#pragma unroll
-                for (int p = 0; p < 4; ++p)
-#pragma unroll
-                    for (int e = 0; e < RUN; ++e)
-                        if (row + 4 * p < rows_left && e < left) at[4 * p * g.ldo + part * (WN / SPLIT) + e] = v[p][e];
-            }
+            to += 4 * row4;
+            row += 16;
+            asm volatile("" : "+v"(to), "+v"(row));  // one address and one row number carried along, not eight of each kept
         }
-        at += 16 * g.ldo;
-        row += 16;
-        asm volatile("" : "+v"(at), "+v"(row));  // one address and one row number carried along, not eight of each kept
-    }
+    };
+    if (rows_left >= WM && cols_left >= WN) write_rows(std::true_type{});
+    else if (rows_left > 0 && cols_left > 0) write_rows(std::false_type{});
     if (!has_next) break;
     id = next_id;
     tile = next;
@@ -778,7 +812,7 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
     p.groups = g.groups; p.rows = g.rows; p.N = g.cols; p.K = g.depth;
     const long long row_tiles = most_row_tiles(g.rows, g.groups, 16);
     p.row_tiles = static_cast<int>(row_tiles);
-    p.k_parts = few_rows_k_parts(g.rows < g.groups ? g.rows : row_tiles, p.N, p.K, kFewStep, kFewWaves);
+    p.k_parts = few_rows_k_parts(g.rows < g.groups ? g.rows : row_tiles, p.N, p.K, kFewStep, kFewWaves, 16);
     p.n_parts = p.k_parts < kFewLeast ? kFewLeast / p.k_parts : 1;
     p.tiles_n = ceil_div(p.N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;

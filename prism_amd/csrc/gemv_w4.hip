@@ -342,7 +342,7 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
     const long long row_tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16) : ceil_div(rows, 16ll);
     // Of a group table's tiles about as many exist as there are rows or groups.
     const long long busy = offsets != nullptr ? (rows < groups ? rows : row_tiles) : row_tiles;
-    p.k_parts = few_rows_k_parts(busy, N, K, kW4Block, kW4Waves);
+    p.k_parts = few_rows_k_parts(busy, N, K, kW4Block, kW4Waves, 8);
     p.n_parts = p.k_parts < kW4Few ? kW4Few / p.k_parts : 1;
     p.tiles_n = ceil_div(N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;
