@@ -33,6 +33,15 @@ __device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(uint16_t* p, float v) { *p = to_bf16(v); }
 
+// v_mfma_f32_16x16x32_bf16 on an accumulator in place, from inline assembly: through the builtin the compiler moves
+// accumulators between registers around the instruction (a hundred moves per 32 of them in the general kernel, spills in the
+// big one). It then does not know the result's latency: an accumulator is read by nothing but the same instruction within 64
+// clocks of its last one (grouped_settle), and a register that the vector ALU has just written is not an operand.
+__device__ __forceinline__ void mfma_in_place(f32x4& c, bf16x8 a, bf16x8 b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void grouped_settle() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory"); }
+
 // One problem, as OUT = P Q^T. Element strides; `groups` weight matrices (or, with RAGGED_C, results) `group_stride`
 // elements apart.
 struct GroupedProblem {
@@ -147,14 +156,21 @@ __device__ __forceinline__ void load_operand(uint16_t* tile, const OperandSource
     }
 }
 
-// BM x BN tiles, four waves of BM/2 x BN/2, two LDS stages of 64 c. RAGGED_C: the groups lie along c (grad_b).
-template <int BM, int BN, bool P_TURNED, bool Q_TURNED, bool RAGGED_C, bool ALIGNED, typename OutT>
+// ------------------------------------------------------------------------------------------- the general kernel --
+// 128 x 128 tiles, four waves of 64 x 64, one tile a workgroup: operands of any alignment, and problems with too few big
+// tiles for the chip. RAGGED_C: the groups lie along c (grad_b).
+// ALIGNED: direct-to-LDS loads into a ring of four stages of 64 c, three stages ahead; with at most one workgroup to a CU
+// nothing else hides the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of
+// the 0.3 its matrix instructions and LDS reads take). Else two stages, through registers.
+template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, bool ALIGNED, typename OutT>
 __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
-    constexpr int WAVES = 4, WM = BM / 2, WN = BN / 2, MI = WM / 16, NI = WN / 16;
+    constexpr int BM = 128, BN = 128, WAVES = 4, WM = BM / 2, WN = BN / 2, MI = WM / 16, NI = WN / 16;
+    constexpr int STAGES = ALIGNED ? 4 : 2;
     using PT = OperandTile<BM, P_TURNED, WAVES>;
     using QT = OperandTile<BN, Q_TURNED, WAVES>;
-    __shared__ __attribute__((aligned(1024))) uint16_t Ps[2][PT::ELEMS];
-    __shared__ __attribute__((aligned(1024))) uint16_t Qs[2][QT::ELEMS];
+    constexpr int LOADS = PT::PASSES + QT::PASSES;  // of a wave and stage
+    __shared__ __attribute__((aligned(1024))) uint16_t Ps[STAGES][PT::ELEMS];
+    __shared__ __attribute__((aligned(1024))) uint16_t Qs[STAGES][QT::ELEMS];
 
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -181,36 +197,59 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
     }
     const int wave_m = wave / 2, wave_n = wave % 2;
     f32x4 acc[MI][NI] = {};
-    const int tiles = (ps.depth + kBK - 1) / kBK;
-    auto load = [&](int t) {
-        load_operand<BM, P_TURNED, WAVES, ALIGNED>(Ps[t & 1], ps, t * kBK, wave, lane);
-        load_operand<BN, Q_TURNED, WAVES, ALIGNED>(Qs[t & 1], qs, t * kBK, wave, lane);
+    const int tiles = __builtin_amdgcn_readfirstlane(ps.depth > 0 ? (ps.depth + kBK - 1) / kBK : 1);  // without depth: a stage of zeros
+    auto load = [&](int t) {  // beyond the last: zeros, so that every stage has its loads in flight
+        load_operand<BM, P_TURNED, WAVES, ALIGNED>(Ps[t % STAGES], ps, t * kBK, wave, lane);
+        load_operand<BN, Q_TURNED, WAVES, ALIGNED>(Qs[t % STAGES], qs, t * kBK, wave, lane);
     };
-    auto landed = [&] {
-        asm volatile("" ::: "memory");  // the compiler knows neither the loads' writes to LDS nor what the barrier orders
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+    auto barrier = [&](auto in_flight) {  // of this wave's loads at most so many are still on their way
+        asm volatile("" ::: "memory");    // the compiler knows neither the loads' writes to LDS nor what the barrier orders
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(decltype(in_flight)::value, 0));
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    if (tiles > 0) load(0);
-    landed();
-    for (int t = 0; t < tiles; ++t) {
-        if (t + 1 < tiles) load(t + 1);
+    auto multiply = [&](int t) {
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             bf16x8 fp[MI], fq[NI];
 #pragma unroll
-            for (int i = 0; i < MI; ++i) fp[i] = PT::fragment(Ps[t & 1], wave_m * WM + i * 16, kk * 32, lane);
+            for (int i = 0; i < MI; ++i) fp[i] = PT::fragment(Ps[t % STAGES], wave_m * WM + i * 16, kk * 32, lane);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) fq[j] = QT::fragment(Qs[t & 1], wave_n * WN + j * 16, kk * 32, lane);
+            for (int j = 0; j < NI; ++j) fq[j] = QT::fragment(Qs[t % STAGES], wave_n * WN + j * 16, kk * 32, lane);
             // Q first: a lane then holds four consecutive columns of one row of OUT.
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fq[j], fp[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < NI; ++j) mfma_in_place(acc[i][j], fq[j], fp[i]);
         }
-        landed();
+    };
+    using none = std::integral_constant<int, 0>;
+    if constexpr (ALIGNED) {
+        // The barrier in front of stage t: it has landed, and everybody is done with stage t - 1, whose place t + 3 takes.
+#pragma unroll
+        for (int t = 0; t < STAGES - 1; ++t) load(t);
+        int t = 0;
+        do {
+            barrier(std::integral_constant<int, (STAGES - 2) * LOADS>{});
+            load(t + STAGES - 1);
+            multiply(t);
+        } while (++t < tiles);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));  // the loads beyond the last stage write LDS
+    } else {
+        load(0);
+        barrier(none{});
+        int t = 0;
+        do {
+            if (t + 1 < tiles) load(t + 1);
+            multiply(t);
+            barrier(none{});
+        } while (++t < tiles);
     }
+    grouped_settle();
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));  // every later use comes behind the wait
     const int cols_left = g.cols - col0;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -219,9 +258,16 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
             const int col = wave_n * WN + j * 16 + 4 * (lane >> 4);
+            OutT* at = out + row * g.ldo + col;
+            if (col + 4 <= cols_left) {
+                typedef OutT Out4 __attribute__((ext_vector_type(4), aligned(sizeof(OutT))));
+                if constexpr (sizeof(OutT) == 4) *reinterpret_cast<Out4*>(at) = acc[i][j];
+                else *reinterpret_cast<Out4*>(at) = Out4{to_bf16(acc[i][j][0]), to_bf16(acc[i][j][1]), to_bf16(acc[i][j][2]), to_bf16(acc[i][j][3])};
+            } else {
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                if (col + v < cols_left) store_out(out + row * g.ldo + col + v, acc[i][j][v]);
+                for (int v = 0; v < 4; ++v)
+                    if (col + v < cols_left) store_out(at + v, acc[i][j][v]);
+            }
         }
     }
 }
@@ -239,11 +285,6 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
 // New here: every load goes through its descriptor's extent, which ends with the group (straight: the lines that exist;
 // turned: the c that exist), so that ragged tiles need no code of their own, and the walk over the tiles of all groups
 // reads a table that the workgroup makes of the offsets in LDS at its start.
-__device__ __forceinline__ void mfma_in_place(f32x4& c, bf16x8 a, bf16x8 b) {
-    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-}
-__device__ __forceinline__ void grouped_settle() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory"); }
-
 // On the scalar ALU by name: a minimum inside a maximum becomes v_med3_i32 otherwise, and a descriptor with a word from
 // the vector ALU cannot be an operand of the load.
 __device__ __forceinline__ int scalar_min(int a, int b) {
@@ -821,38 +862,58 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
     return check_launch("gemm_grouped_few_kernel");
 }
 
-// Whether 256 x 256 tiles are worth it: enough rows a group to fill them.
-bool big_pays(const GroupedProblem& g, bool ragged_c) {
-    if (g.groups > kBigGroups || cu_count() < 8) return false;
-    if (!ragged_c) return g.rows / g.groups >= 160;
-    return g.rows / g.groups >= 128;
+// Which kernel: the one with the smallest estimate, in us, of these simple costs (all figures measured on one MI355X with
+// 32 or fewer groups; `used` groups have rows, which the host takes to be as many as there can be, and a group wastes half a
+// row tile):
+//   few      7 + B read once per 16-row tile at 4.7 TB/s
+//   general  rounds of 256 tiles of 128 x 128 at 4 + 0.48 a stage, or B once at 4.3 TB/s
+//   big      rounds of 256 tiles of 256 x 256 at 8 + 1.2 a stage (stages in pairs), or B once at 4.3 TB/s
+// Measured, few / general / big: 64 rows of 32 groups, 2048 x 2048: 56 / 57 / 65 us; 512 rows: 101 / 63 / 70; 2048 rows:
+// 252 / 67 / 73; 8192 rows: - / 106 / 82; 100 rows of 8 groups, 256 x 4096: 10 / 34 / 69; 2000 rows of 16, 768 x 768: 38 /
+// 12 / 21. Gradient of B, general / big: 512 rows of 32 groups, 2048 x 2048: 137 / 66; 1000 rows of 32, 304 x 512: 10 / 12.
+enum class Kernel { kFew, kGeneral, kBig };
+template <bool RAGGED_C>
+Kernel choose_kernel(const GroupedProblem& g, bool can_few, bool can_big) {
+    const double rows = g.rows, groups = g.groups, used = rows < groups ? rows : groups;
+    auto row_tiles = [&](double tile) { const double t = rows / tile + used / 2; return t > used ? t : used; };
+    auto rounds = [](double tiles) { return static_cast<double>(static_cast<long long>((tiles + 255.0) / 256.0)); };
+    const double depth = RAGGED_C ? rows / groups : static_cast<double>(g.depth), stages = static_cast<double>(static_cast<long long>((depth + 63) / 64));
+    const double b_us = RAGGED_C ? 0.0 : used * g.cols * depth * 2 / 4.3e6;
+    auto tiled = [&](int edge, double fixed, double stage_us, double n_stages) {
+        const double tiles = (RAGGED_C ? groups * ceil_div(g.out_rows, edge) : row_tiles(edge)) * ceil_div(g.cols, edge);
+        const double us = rounds(tiles) * (fixed + stage_us * n_stages);
+        return 2 + (us > b_us ? us : b_us);
+    };
+    const double general = tiled(128, 4, 0.48, stages > 1 ? stages : 1);
+    const double big = can_big ? tiled(256, 8, 1.2, stages > 2 ? stages + static_cast<long long>(stages) % 2 : 2) : 1e30;
+    const double few = can_few ? 7 + row_tiles(16) * g.cols * depth * 2 / 4.7e6 : 1e30;
+    if (few <= general && few <= big) return Kernel::kFew;
+    return general <= big ? Kernel::kGeneral : Kernel::kBig;
 }
-
-// Whether tiles of 16 rows are worth it: a group's weights are read once per tile.
-bool few_pays(const GroupedProblem& g) { return g.rows / g.groups <= 16; }
 
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
 int run(GroupedProblem g, const char* who, hipStream_t s) {
-    constexpr int BM = 128, BN = 128;
-    if constexpr (!P_TURNED && !Q_TURNED)
-        if (few_pays(g)) return run_few<OutT>(g, who, s);
-    g.tiles_n = ceil_div(g.cols, BN);
-    const long long tiles_m = RAGGED_C ? static_cast<long long>(g.groups) * ceil_div(g.out_rows, BM) : most_row_tiles(g.rows, g.groups, BM);
-    if (tiles_m == 0) return 0;
-    if (tiles_m * g.tiles_n > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
-    const dim3 grid(static_cast<unsigned>(tiles_m * g.tiles_n));
+    constexpr bool FORWARD = !P_TURNED && !Q_TURNED;
     // Direct-to-LDS loads need 16 B chunks that are whole or absent (bases, strides and the extents along memory in
-    // multiples of 8 elements) and 32-bit offsets inside a tile.
+    // multiples of 8 elements) and 32-bit offsets inside a tile. What is not aligned runs on the general kernel, or on the
+    // one for few rows, which reads B where it lies.
     const int p_along = P_TURNED ? g.out_rows : g.depth, q_along = Q_TURNED ? g.cols : g.depth;
     const bool aligned = aligned16(g.P) && aligned16(g.Q) && g.ldp % 8 == 0 && g.ldq % 8 == 0 && (RAGGED_C || g.group_stride % 8 == 0) &&
                          p_along % 8 == 0 && q_along % 8 == 0 && g.ldp < (1 << 21) && g.ldq < (1 << 21);
-    if (aligned && big_pays(g, RAGGED_C)) {
-        g.tiles_n = ceil_div(g.cols, 256);
+    const Kernel kernel = choose_kernel<RAGGED_C>(g, FORWARD, aligned && g.groups <= kBigGroups && cu_count() >= 8);
+    if constexpr (FORWARD)
+        if (kernel == Kernel::kFew) return run_few<OutT>(g, who, s);
+    const int edge = kernel == Kernel::kBig ? 256 : 128;
+    g.tiles_n = ceil_div(g.cols, edge);
+    const long long tiles_m = RAGGED_C ? static_cast<long long>(g.groups) * ceil_div(g.out_rows, edge) : most_row_tiles(g.rows, g.groups, edge);
+    if (tiles_m * g.tiles_n > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
+    if (kernel == Kernel::kBig) {
         gemm_grouped_big_kernel<P_TURNED, Q_TURNED, RAGGED_C, OutT><<<dim3(static_cast<unsigned>(cu_count() / 8 * 8)), dim3(256), 0, s>>>(g);
         return check_launch("gemm_grouped_big_kernel");
     }
-    if (aligned) gemm_grouped_kernel<BM, BN, P_TURNED, Q_TURNED, RAGGED_C, true, OutT><<<grid, dim3(256), 0, s>>>(g);
-    else gemm_grouped_kernel<BM, BN, P_TURNED, Q_TURNED, RAGGED_C, false, OutT><<<grid, dim3(256), 0, s>>>(g);
+    const dim3 grid(static_cast<unsigned>(tiles_m * g.tiles_n));
+    if (aligned) gemm_grouped_kernel<P_TURNED, Q_TURNED, RAGGED_C, true, OutT><<<grid, dim3(256), 0, s>>>(g);
+    else gemm_grouped_kernel<P_TURNED, Q_TURNED, RAGGED_C, false, OutT><<<grid, dim3(256), 0, s>>>(g);
     return check_launch("gemm_grouped_kernel");
 }
 

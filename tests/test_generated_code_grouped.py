@@ -27,8 +27,8 @@ def test_direct_loads(text):
 
 
 def test_matrix_instructions(text):
-    """The accumulator check goes by its kernel's name: the grouped kernel is shown to it under that name."""
-    shown = {"gemm_bf16.hip": text.replace("gemm_grouped_big_kernel", "gemm_bf16_early_kernel")}
+    """The accumulator check goes by its kernel's name: the grouped kernels are shown to it under that name."""
+    shown = {"gemm_bf16.hip": re.sub(r"gemm_grouped(_big)?_kernel", "gemm_bf16_early_kernel", text)}
     gen.test_no_matrix_instruction_reads_a_register_the_vector_alu_has_just_written(shown)
     gen.test_no_accumulator_is_read_too_soon_after_an_in_place_matrix_instruction(shown)
 

@@ -97,7 +97,8 @@ def test_grouped_products_strides_and_alignments(prism, sizes, n, k, start, pad)
 
 
 @pytest.mark.parametrize("sizes,n,k", [([900, 1100, 40, 700], 1024, 1536), ([513] * 12, 768, 512), ([2048, 0, 2500], 2048, 640), ([130] * 40, 520, 328),
-                                       ([3000, 5000], 1500, 1032), ([60] * 64, 512, 256), ([20] * 100, 384, 640)], ids=lambda v: str(len(v)) if isinstance(v, list) else str(v))
+                                       ([3000, 5000], 1500, 1032), ([60] * 64, 512, 256), ([20] * 100, 384, 640),
+                                       ([2500, 1300, 0, 3100, 700, 1], 1536, 512), ([1700, 2300, 1800, 2222, 257], 1400, 520), ([129] * 33 + [900], 1288, 2056)], ids=lambda v: str(len(v)) if isinstance(v, list) else str(v))
 def test_grouped_products_with_more_tiles_than_workgroups(prism, sizes, n, k):
     grouped_case(prism, sizes, n, k, torch.bfloat16, seed=n, behind=7)
     grouped_case(prism, sizes, n, k, torch.float32, seed=n + 1)
