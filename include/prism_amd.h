@@ -435,6 +435,15 @@ int prism_expert_plan(const int32_t* chosen, int64_t tokens, int k, int experts,
                       void* stream);
 
 /*
+ * prism_route_topk and prism_expert_plan of its choice in one call, in as few
+ * launches as they take together (one up to 64 tokens). Arguments and workspace
+ * as there.
+ */
+int prism_route_plan(const void* logits, int type, int64_t ld, int64_t tokens, int experts, int k,
+                     int renormalise, float* weights, int32_t* chosen, int32_t* offsets, int32_t* rows,
+                     int32_t* slots, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * out[s] = x[rows[s] / k] for the n_slots slots with rows[s] >= 0 (the others
  * are left as they are). x: tokens x width, out: n_slots x width, both of
  * `type`. Its gradient is prism_expert_combine with weights == NULL.

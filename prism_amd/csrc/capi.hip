@@ -207,6 +207,12 @@ int prism_route_topk(const void* logits, int type, int64_t ld, int64_t tokens, i
     return launch_route_topk(type, logits, ld, tokens, experts, k, renormalise, weights, chosen, static_cast<hipStream_t>(stream));
 }
 
+int prism_route_plan(const void* logits, int type, int64_t ld, int64_t tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
+                     int32_t* offsets, int32_t* rows, int32_t* slots, void* workspace, size_t workspace_bytes, void* stream) {
+    return launch_route_plan(type, logits, ld, tokens, experts, k, renormalise, weights, chosen, offsets, rows, slots, workspace, workspace_bytes,
+                             static_cast<hipStream_t>(stream));
+}
+
 int prism_route_topk_backward(const float* grad_weights, const void* logits, int type, int64_t ld, const float* weights, const int32_t* chosen,
                               int64_t tokens, int experts, int k, int renormalise, void* grad_logits, int64_t ld_grad, void* stream) {
     return launch_route_backward(type, grad_weights, logits, ld, weights, chosen, tokens, experts, k, renormalise, grad_logits, ld_grad,

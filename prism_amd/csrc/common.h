@@ -99,6 +99,9 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
                    const uint16_t* scales, const uint8_t* zeros, int group_size, const int32_t* offsets, void* y, long long ldy, int out_type, hipStream_t s);
 int launch_route_topk(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
                       hipStream_t s);
+// The choice and its plan in as few launches as they take together.
+int launch_route_plan(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
+                      int32_t* offsets, int32_t* rows, int32_t* slots, void* ws, size_t ws_bytes, hipStream_t s);
 int launch_route_backward(int type, const float* grad, const void* logits, long long ld, const float* weights, const int32_t* chosen, long long tokens,
                           int experts, int k, int renormalise, void* out, long long ldo, hipStream_t s);
 size_t expert_plan_workspace_bytes(long long tokens, int k, int experts);

@@ -865,7 +865,7 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
 // Which kernel: the one with the smallest estimate, in us, of these simple costs (all figures measured on one MI355X with
 // 32 or fewer groups; `used` groups have rows, which the host takes to be as many as there can be, and a group wastes half a
 // row tile):
-//   few      7 + B read once per 16-row tile at 4.7 TB/s
+//   few      5 + B read once per 16-row tile at 5.3 TB/s with up to 4 rows a group, 3.9 with more (see instruction_x)
 //   general  rounds of 256 tiles of 128 x 128 at 4 + 0.48 a stage, or B once at 4.3 TB/s
 //   big      rounds of 256 tiles of 256 x 256 at 8 + 1.2 a stage (stages in pairs), or B once at 4.3 TB/s
 // Measured, few / general / big: 64 rows of 32 groups, 2048 x 2048: 56 / 57 / 65 us; 512 rows: 101 / 63 / 70; 2048 rows:
@@ -886,7 +886,7 @@ Kernel choose_kernel(const GroupedProblem& g, bool can_few, bool can_big) {
     };
     const double general = tiled(128, 4, 0.48, stages > 1 ? stages : 1);
     const double big = can_big ? tiled(256, 8, 1.2, stages > 2 ? stages + static_cast<long long>(stages) % 2 : 2) : 1e30;
-    const double few = can_few ? 7 + row_tiles(16) * g.cols * depth * 2 / 4.7e6 : 1e30;
+    const double few = can_few ? 5 + row_tiles(16) * g.cols * depth * 2 / (rows <= 4 * groups ? 5.3e6 : 3.9e6) : 1e30;
     if (few <= general && few <= big) return Kernel::kFew;
     return general <= big ? Kernel::kGeneral : Kernel::kBig;
 }

@@ -17,117 +17,188 @@
 namespace prism {
 namespace {
 
-constexpr int kRouteBlock = 256;
 constexpr int kMaxExperts = 1024, kMaxChosen = 32;
+constexpr int kLanes = 16;  // lanes of a token: a DPP row, so that its sums and maxima need no LDS
 
-__device__ __forceinline__ float load_logit(const float* p) { return *p; }
-__device__ __forceinline__ float load_logit(const uint16_t* p) { return __builtin_bit_cast(float, static_cast<uint32_t>(*p) << 16); }
-__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Logits as unsigned integers of the same order: -0 as 0, any NaN above +inf.
+template <int N>
+__device__ __forceinline__ uint32_t rotated(uint32_t v) { return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, true); }  // row_ror
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max(v, rotated<8>(v));
+    v = max(v, rotated<4>(v));
+    v = max(v, rotated<2>(v));
+    return max(v, rotated<1>(v));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    auto turn = [](uint32_t u) { return __builtin_bit_cast(float, u); };
+    auto bits = [](float f) { return __builtin_bit_cast(uint32_t, f); };
+    v += turn(rotated<8>(bits(v)));
+    v += turn(rotated<4>(bits(v)));
+    v += turn(rotated<2>(bits(v)));
+    return v + turn(rotated<1>(bits(v)));
+}
+// Lane 0's value of every row.
+__device__ __forceinline__ uint32_t row_first(uint32_t v) { return __builtin_amdgcn_update_dpp(0, v, 0x150, 0xf, 0xf, true); }
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(uint16_t v) { return __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16); }
+__device__ __forceinline__ void from_float(float& to, float v) { to = v; }
+__device__ __forceinline__ void from_float(uint16_t& to, float v) { to = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }  // nearest even
+
+// PACK consecutive values in one access (16 B, or one value).
+template <typename T, int PACK>
+struct Logits {
+    T v[PACK];
+    static __device__ __forceinline__ Logits load(const T* p) {
+        Logits r;
+        __builtin_memcpy(r.v, __builtin_assume_aligned(p, PACK * sizeof(T)), PACK * sizeof(T));
+        return r;
+    }
+    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(__builtin_assume_aligned(p, PACK * sizeof(T)), v, PACK * sizeof(T)); }
+};
+
+// Logits as unsigned integers of the same order: -0 as 0, any NaN above +inf. bf16 logits leave the lower 16 bits free.
 __device__ __forceinline__ uint32_t order_of(float z) {
     z += 0.0f;
-    const uint32_t u = z != z ? 0x7fffffffu : __builtin_bit_cast(uint32_t, z);
+    const uint32_t u = z != z ? 0x7fff0000u : __builtin_bit_cast(uint32_t, z);
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of(uint32_t o) { return __builtin_bit_cast(float, (o & 0x80000000u) ? o & 0x7fffffffu : ~o); }
 constexpr uint32_t kOrderNone = 0x007fffffu;  // order_of(-inf): this and below is not there
 
-// One token by LANES consecutive lanes, VALUES logits each (lane i has experts i, i + LANES, ...).
-template <typename T, int LANES, int VALUES>
+// One token by the 16 lanes of a row, VALUES logits each: value v of a lane is expert (v / PACK) 16 PACK + lane PACK + v % PACK.
+// Picking is k rounds of: the row's largest key, its expert, its key struck out. bf16: the key holds the order in its upper
+// half and the complement of the expert in its lower one, so that one maximum finds both; fp32: the order is the key, the
+// lowest expert that has it is found by a second maximum (of complements).
+template <typename T, int VALUES, int PACK>
 __device__ __forceinline__ void choose_experts(const T* z, int experts, int k, bool renormalise, float* weights, int32_t* chosen) {
-    const int lane = threadIdx.x & (LANES - 1);
-    uint32_t order[VALUES];
-    float logit[VALUES];
+    constexpr bool PACKED = sizeof(T) == 2;
+    const int lane = threadIdx.x & (kLanes - 1);
+    auto expert_of = [&](int v) { return (v / PACK) * (kLanes * PACK) + lane * PACK + v % PACK; };
+    uint32_t key[VALUES];
 #pragma unroll
-    for (int v = 0; v < VALUES; ++v) {
-        const int e = lane + v * LANES;
-        logit[v] = e < experts ? load_logit(z + e) : -INFINITY;
-        order[v] = order_of(logit[v]);
-    }
-    // The chosen ones, one after the other: lane j (and j - LANES) keeps the j-th.
-    constexpr int KEEP = kMaxChosen / LANES > 0 ? kMaxChosen / LANES : 1;
-    uint32_t my_order[KEEP];
-    int my_expert[KEEP];
+    for (int v = 0; v < VALUES; v += PACK) {
+        const int e = expert_of(v);
+        if (e < experts) {
+            const Logits<T, PACK> at = Logits<T, PACK>::load(z + e);
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) { my_order[i] = kOrderNone; my_expert[i] = -1; }
-    uint32_t top = kOrderNone;
-    for (int j = 0; j < k; ++j) {
-        uint32_t best = 0;
-        int at = 0;
+            for (int i = 0; i < PACK; ++i) {
+                const uint32_t o = order_of(as_float(at.v[i]));
+                key[v + i] = o <= kOrderNone ? 0u : (PACKED ? (o & 0xffff0000u) | static_cast<uint16_t>(~(e + i)) : o);
+            }
+        } else {
 #pragma unroll
-        for (int v = 0; v < VALUES; ++v)
-            if (order[v] > best) { best = order[v]; at = v; }  // strictly: the lower index stays
-        unsigned long long key = (static_cast<unsigned long long>(best) << 32) | static_cast<uint32_t>(~(lane + at * LANES));
-#pragma unroll
-        for (int d = LANES / 2; d > 0; d /= 2) {
-            const unsigned long long other = __shfl_xor(key, d);
-            key = other > key ? other : key;
+            for (int i = 0; i < PACK; ++i) key[v + i] = 0u;
         }
-        const uint32_t won = static_cast<uint32_t>(key >> 32);
-        if (won <= kOrderNone) break;  // the same for all LANES lanes
-        const int expert = static_cast<int>(~static_cast<uint32_t>(key));
+    }
+    // Lane j keeps the j-th and the (j + 16)-th.
+    uint32_t my_key[2] = {0u, 0u};
+    int my_expert[2] = {-1, -1};
+    uint32_t top = 0;
+    for (int j = 0; j < k; ++j) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int v = 1; v < VALUES; ++v) best = max(best, key[v]);
+        const uint32_t won = row_max(best);
+        if (won == 0) break;  // the same for the 16 lanes
+        int expert;
+        if constexpr (PACKED) {
+            expert = static_cast<uint16_t>(~won);
+#pragma unroll
+            for (int v = 0; v < VALUES; ++v) key[v] = key[v] == won ? 0u : key[v];  // keys differ: it is this expert's
+        } else {
+            uint32_t other = 0;  // complement of the lowest expert with this order, among this lane's
+#pragma unroll
+            for (int v = VALUES - 1; v >= 0; --v) other = key[v] == won ? ~static_cast<uint32_t>(expert_of(v)) : other;
+            expert = static_cast<int>(~row_max(other));
+#pragma unroll
+            for (int v = 0; v < VALUES; ++v) key[v] = expert_of(v) == expert ? 0u : key[v];
+        }
         if (j == 0) top = won;
 #pragma unroll
-        for (int i = 0; i < KEEP; ++i)
-            if (j == lane + i * LANES) { my_order[i] = won; my_expert[i] = expert; }
-#pragma unroll
-        for (int v = 0; v < VALUES; ++v)
-            if (lane + v * LANES == expert) order[v] = 0;
+        for (int i = 0; i < 2; ++i)
+            if (j == lane + i * kLanes) { my_key[i] = won; my_expert[i] = expert; }
     }
-    const float z0 = logit_of(top);
-    float total = 0.0f, up[KEEP];
+    // (the order of a negative bf16 logit has ones in its lower half)
+    auto logit = [](uint32_t o) { return logit_of(!PACKED ? o : ((o & 0x80000000u) ? o & 0xffff0000u : o | 0xffffu)); };
+    const float z0 = logit(top);
+    float total = 0.0f, up[2];
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-        up[i] = my_order[i] > kOrderNone ? expf(logit_of(my_order[i]) - z0) : 0.0f;
-        if (renormalise) total += up[i];
+    for (int i = 0; i < 2; ++i) {
+        up[i] = my_key[i] ? expf(logit(my_key[i]) - z0) : 0.0f;
+        total += up[i];
     }
-    if (!renormalise && top > kOrderNone)
+    if (!renormalise)  // and those that were not chosen
 #pragma unroll
-        for (int v = 0; v < VALUES; ++v) total += logit[v] == -INFINITY ? 0.0f : expf(logit[v] - z0);
+        for (int v = 0; v < VALUES; ++v) total += key[v] ? expf(logit(key[v]) - z0) : 0.0f;
+    total = row_sum(total);
 #pragma unroll
-    for (int d = LANES / 2; d > 0; d /= 2) total += __shfl_xor(total, d);
-#pragma unroll
-    for (int i = 0; i < KEEP; ++i) {
-        const int j = lane + i * LANES;
+    for (int i = 0; i < 2; ++i) {
+        const int j = lane + i * kLanes;
         if (j < k) {
-            weights[j] = my_order[i] > kOrderNone ? up[i] / total : 0.0f;
+            weights[j] = my_key[i] ? up[i] / total : 0.0f;
             chosen[j] = my_expert[i];
         }
     }
 }
 
-template <typename T, int LANES, int VALUES>
+constexpr int kRouteBlock = 256;
+
+template <typename T, int VALUES, int PACK>
 __global__ __launch_bounds__(kRouteBlock) void route_topk_kernel(const T* __restrict__ logits, long long ld, int tokens, int experts, int k,
                                                                  int renormalise, float* __restrict__ weights, int32_t* __restrict__ chosen) {
-    const int token = blockIdx.x * (kRouteBlock / LANES) + threadIdx.x / LANES;
-    if (token >= tokens) return;  // whole groups of LANES lanes
+    const int token = blockIdx.x * (kRouteBlock / kLanes) + threadIdx.x / kLanes;
+    if (token >= tokens) return;  // whole rows of lanes
     const long long at = static_cast<long long>(token) * k;
-    choose_experts<T, LANES, VALUES>(logits + token * ld, experts, k, renormalise != 0, weights + at, chosen + at);
+    choose_experts<T, VALUES, PACK>(logits + token * ld, experts, k, renormalise != 0, weights + at, chosen + at);
 }
 
-// One thread group of 16 lanes per token.
-template <typename T>
+// 16 lanes a token: the gradient as if nothing had been chosen (0, or -c p_e), then the chosen experts' over it: every
+// w_j (g_j - c), since p_e = w_j for a chosen expert of weights that are not renormalised.
+template <typename T, int PACK>
 __global__ __launch_bounds__(kRouteBlock) void route_backward_kernel(const float* __restrict__ grad, const T* __restrict__ logits, long long ld,
                                                                      const float* __restrict__ weights, const int32_t* __restrict__ chosen,
-                                                                     int tokens, int experts, int k, int renormalise, T* __restrict__ out, long long ldo) {
-    const int token = blockIdx.x * (kRouteBlock / 16) + threadIdx.x / 16;
+                                                                     int tokens, int experts, int k, int renormalise, T* out, long long ldo) {
+    const int token = blockIdx.x * (kRouteBlock / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x & (kLanes - 1);
     if (token >= tokens) return;
     const long long at = static_cast<long long>(token) * k;
-    float c = 0.0f;
-    for (int j = 0; j < k; ++j)
-        if (chosen[at + j] >= 0) c = __builtin_fmaf(weights[at + j], grad[at + j], c);
-    const int first = chosen[at];
-    const bool any = first >= 0 && first < experts;
-    const float w0 = any ? weights[at] : 0.0f, z0 = any && !renormalise ? load_logit(logits + token * ld + first) : 0.0f;
-    for (int e = threadIdx.x & 15; e < experts; e += 16) {
-        float d = 0.0f;
-        if (!renormalise && any) d = -c * w0 * expf(load_logit(logits + token * ld + e) - z0);
-        for (int j = 0; j < k; ++j)
-            if (chosen[at + j] == e) d = renormalise ? weights[at + j] * (grad[at + j] - c) : __builtin_fmaf(weights[at + j], grad[at + j], d);
-        store_logit(out + token * ldo + e, d);
+    const T* z = logits + token * ld;
+    T* to = out + token * ldo;
+    float w[2], g[2], c = 0.0f;
+    int e[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = lane + i * kLanes;
+        e[i] = j < k ? chosen[at + j] : -1;
+        const bool there = e[i] >= 0 && e[i] < experts;
+        w[i] = there ? weights[at + j] : 0.0f;
+        g[i] = there ? grad[at + j] : 0.0f;
+        if (!there) e[i] = -1;
+        c = __builtin_fmaf(w[i], g[i], c);
     }
+    c = row_sum(c);
+    const int first = static_cast<int>(row_first(static_cast<uint32_t>(e[0])));
+    const bool dense = !renormalise && first >= 0;  // else zeros
+    const float w0 = __builtin_bit_cast(float, row_first(__builtin_bit_cast(uint32_t, w[0])));
+    const float z0 = dense ? as_float(z[first]) : 0.0f, scale = -c * w0;
+    for (int i = lane * PACK; i < experts; i += kLanes * PACK) {
+        Logits<T, PACK> d;
+        if (dense) {
+            const Logits<T, PACK> v = Logits<T, PACK>::load(z + i);
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) from_float(d.v[j], scale * expf(as_float(v.v[j]) - z0));
+        } else {
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) from_float(d.v[j], 0.0f);
+        }
+        d.store(to + i);
+    }
+    // The same wavefront writes these again: behind its first stores.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (e[i] >= 0) from_float(to[e[i]], w[i] * (g[i] - c));
 }
 
 // ------------------------------------------------------------------------------------------------------------ plan --
@@ -194,115 +265,166 @@ __device__ __forceinline__ void scan_experts(int* value, int experts) {
 }
 
 // One workgroup does the whole plan up to here: its counters fit 64 KiB of LDS.
-constexpr int kSmallWaves = 16, kSmallEntries = 4096, kSmallExperts = 512;
-inline bool one_workgroup(long long entries, int experts) { return entries <= kSmallEntries && experts <= kSmallExperts; }
+// One workgroup of 16 wavefronts does a run of up to kRun entries: counts them per wavefront in LDS, sums the counts over
+// the wavefronts, places them. A plan of one run takes the experts' offsets from its own counts; in longer ones they come
+// from the counts of all runs (plan_count_kernel), which every run adds up for itself, or, with many runs, plan_sum_kernel.
+constexpr int kRunWaves = 16, kRun = 4096, kShortRun = 512;
+constexpr int kSelfSum = 32;  // runs up to which each adds up all counts
 
-// The plan by one workgroup of 16 wavefronts: counts per wavefront, sums over wavefronts and experts, places.
-__device__ __forceinline__ void plan_in_workgroup(const int32_t* chosen, int entries, int experts, int bits, int32_t* offsets, int32_t* rows,
-                                                  int32_t* slots, int* lds /* (16 + 1) * experts + 1 */) {
-    int* count = lds;                              // [wave][expert]
-    int* total = lds + kSmallWaves * experts;      // [expert + 1]
+__device__ __forceinline__ void count_run(const int32_t* chosen, int first, int end, int per, int experts, int* count) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    for (int i = threadIdx.x; i < kSmallWaves * experts; i += blockDim.x) count[i] = 0;
+    for (int i = threadIdx.x; i < kRunWaves * experts; i += blockDim.x) count[i] = 0;
     __syncthreads();
-    const int per = (entries + kSmallWaves * kWave - 1) / (kSmallWaves * kWave) * kWave;
-    const int first = min(wave * per, entries), end = min(first + per, entries);
-    for (int base = first; base < end; base += kWave) {
-        const int mine = entry_expert(chosen, base + lane, end, experts);
-        if (mine >= 0) atomicAdd(&count[wave * experts + mine], 1);
+    for (int base = first + wave * per; base < min(first + (wave + 1) * per, end); base += kWave) {
+        const int mine = entry_expert(chosen, base + lane, min(first + (wave + 1) * per, end), experts);
+        if (mine >= 0) atomicAdd(&count[wave * experts + mine], 1);  // sums of ones: no order
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-        int sum = 0;
-        for (int w = 0; w < kSmallWaves; ++w) {
-            const int c = count[w * experts + e];
-            count[w * experts + e] = sum;
-            sum += c;
-        }
-        total[e] = sum;
-    }
-    __syncthreads();
-    scan_experts(total, experts);
-    for (int e = threadIdx.x; e < experts; e += blockDim.x)
-        for (int w = 0; w < kSmallWaves; ++w) count[w * experts + e] += total[e];
-    for (int e = threadIdx.x; e <= experts; e += blockDim.x) offsets[e] = total[e];
-    __syncthreads();
-    for (int i = total[experts] + threadIdx.x; i < entries; i += blockDim.x) rows[i] = -1;
-    place_chunk(chosen, first, end, experts, bits, count + wave * experts, rows, slots);
 }
 
-__global__ __launch_bounds__(kSmallWaves * kWave) void plan_small_kernel(const int32_t* chosen, int entries, int experts, int bits, int32_t* offsets,
-                                                                          int32_t* rows, int32_t* slots) {
+// count[wave][expert] becomes the next slot of every wavefront and expert, given start[expert], the run's own first slots.
+__device__ __forceinline__ void place_run(const int32_t* chosen, int first, int end, int per, int experts, int bits, int* count, const int* start,
+                                          int total, int32_t* rows, int32_t* slots) {
+    const int wave = threadIdx.x / kWave;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        int next = start[e];
+        for (int w = 0; w < kRunWaves; ++w) {
+            const int c = count[w * experts + e];
+            count[w * experts + e] = next;
+            next += c;
+        }
+    }
+    __syncthreads();
+    for (int i = max(first, total) + threadIdx.x; i < end; i += blockDim.x) rows[i] = -1;  // slots that are not used
+    place_chunk(chosen, min(first + wave * per, end), min(first + (wave + 1) * per, end), experts, bits, count + wave * experts, rows, slots);
+}
+
+__device__ __forceinline__ int per_wave(int run) { return (run + kRunWaves * kWave - 1) / (kRunWaves * kWave) * kWave; }
+
+// A whole plan by one workgroup. lds: (16 + 1) * experts + 1 ints.
+__device__ __forceinline__ void plan_in_workgroup(const int32_t* chosen, int entries, int experts, int bits, int32_t* offsets, int32_t* rows,
+                                                  int32_t* slots, int* lds) {
+    int *count = lds, *start = lds + kRunWaves * experts;
+    const int per = per_wave(entries);
+    count_run(chosen, 0, entries, per, experts, count);
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        int sum = 0;
+        for (int w = 0; w < kRunWaves; ++w) sum += count[w * experts + e];
+        start[e] = sum;
+    }
+    __syncthreads();
+    scan_experts(start, experts);
+    for (int e = threadIdx.x; e <= experts; e += blockDim.x) offsets[e] = start[e];
+    place_run(chosen, 0, entries, per, experts, bits, count, start, start[experts], rows, slots);
+}
+
+__global__ __launch_bounds__(kRunWaves * kWave) void plan_small_kernel(const int32_t* chosen, int entries, int experts, int bits, int32_t* offsets,
+                                                                       int32_t* rows, int32_t* slots) {
     extern __shared__ int plan_lds[];
     plan_in_workgroup(chosen, entries, experts, bits, offsets, rows, slots, plan_lds);
 }
 
-// Larger plans: chunks of kChunk entries, one per wavefront. counts[chunk][expert], then its exclusive sums over the
-// chunks and the experts' totals, then the places.
-constexpr int kChunk = 512, kChunkWaves = 4;
-
-__global__ __launch_bounds__(kChunkWaves * kWave) void plan_count_kernel(const int32_t* __restrict__ chosen, int entries, int experts, int* __restrict__ counts) {
+// Router and plan of up to 64 tokens (16 lanes each) in one launch.
+template <typename T, int VALUES, int PACK>
+__global__ __launch_bounds__(kRunWaves * kWave) void route_small_kernel(const T* logits, long long ld, int tokens, int experts, int k, int renormalise,
+                                                                        float* weights, int32_t* chosen, int bits, int32_t* offsets, int32_t* rows,
+                                                                        int32_t* slots) {
     extern __shared__ int plan_lds[];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    for (int i = threadIdx.x; i < kChunkWaves * experts; i += blockDim.x) plan_lds[i] = 0;
-    __syncthreads();
-    const int chunk = blockIdx.x * kChunkWaves + wave;
-    const long long first = static_cast<long long>(chunk) * kChunk;
-    if (first < entries) {
-        const int end = static_cast<int>(first + kChunk < entries ? first + kChunk : entries);
-        for (int base = static_cast<int>(first); base < end; base += kWave) {
-            const int mine = entry_expert(chosen, base + lane, end, experts);
-            if (mine >= 0) atomicAdd(&plan_lds[wave * experts + mine], 1);
-        }
-    }
-    __syncthreads();
-    if (first < entries)
-        for (int e = lane; e < experts; e += kWave) counts[static_cast<long long>(chunk) * experts + e] = plan_lds[wave * experts + e];
+    const int token = threadIdx.x / kLanes;
+    if (token < tokens) choose_experts<T, VALUES, PACK>(logits + token * ld, experts, k, renormalise != 0, weights + token * k, chosen + token * k);
+    __syncthreads();  // what this workgroup wrote to memory it may read behind this
+    plan_in_workgroup(chosen, tokens * k, experts, bits, offsets, rows, slots, plan_lds);
 }
 
-// 16 experts a workgroup, the chunks in 64 runs.
-__global__ __launch_bounds__(1024) void plan_sum_kernel(int* __restrict__ counts, int chunks, int experts, int* __restrict__ totals) {
-    __shared__ int run_sum[64][17];
-    const int e = blockIdx.x * 16 + threadIdx.x % 16, run = threadIdx.x / 16;
-    const int per = (chunks + 63) / 64, first = min(run * per, chunks), end = min(first + per, chunks);
+// counts[run][expert]
+__global__ __launch_bounds__(kRunWaves * kWave) void plan_count_kernel(const int32_t* __restrict__ chosen, int entries, int experts, int run,
+                                                                       int* __restrict__ counts) {
+    extern __shared__ int plan_lds[];
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) plan_lds[e] = 0;
+    __syncthreads();
+    const int first = blockIdx.x * run, end = min(first + run, entries);
+    for (int i = first + threadIdx.x; i < end; i += blockDim.x) {
+        const int mine = entry_expert(chosen, i, end, experts);
+        if (mine >= 0) atomicAdd(&plan_lds[mine], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[static_cast<long long>(blockIdx.x) * experts + e] = plan_lds[e];
+}
+
+// Router of 64 tokens a workgroup, and their counts: the plan's first step rides along.
+template <typename T, int VALUES, int PACK>
+__global__ __launch_bounds__(kRunWaves * kWave) void route_count_kernel(const T* __restrict__ logits, long long ld, int tokens, int experts, int k, int renormalise,
+                                                                        float* weights, int32_t* chosen, int* __restrict__ counts) {
+    extern __shared__ int plan_lds[];
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) plan_lds[e] = 0;
+    const int token0 = blockIdx.x * (kRunWaves * kWave / kLanes), token = token0 + threadIdx.x / kLanes;
+    const long long at = static_cast<long long>(token) * k;
+    if (token < tokens) choose_experts<T, VALUES, PACK>(logits + token * ld, experts, k, renormalise != 0, weights + at, chosen + at);
+    __syncthreads();
+    const int first = token0 * k, end = min(first + kRunWaves * kWave / kLanes * k, tokens * k);
+    for (int i = first + threadIdx.x; i < end; i += blockDim.x) {
+        const int mine = entry_expert(chosen, i, end, experts);
+        if (mine >= 0) atomicAdd(&plan_lds[mine], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[static_cast<long long>(blockIdx.x) * experts + e] = plan_lds[e];
+}
+
+// counts[run][expert] becomes its sum over the runs before; totals[expert] the sum over all. 16 experts a workgroup, the
+// runs in 64 parts.
+__global__ __launch_bounds__(1024) void plan_sum_kernel(int* __restrict__ counts, int runs, int experts, int* __restrict__ totals) {
+    __shared__ int part_sum[64][17];
+    const int e = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16;
+    const int per = (runs + 63) / 64, first = min(part * per, runs), end = min(first + per, runs);
     int sum = 0;
     if (e < experts)
         for (int c = first; c < end; ++c) sum += counts[static_cast<long long>(c) * experts + e];
-    run_sum[run][threadIdx.x % 16] = sum;
+    part_sum[part][threadIdx.x % 16] = sum;
     __syncthreads();
     if (e >= experts) return;
     int before = 0;
-    for (int r = 0; r < run; ++r) before += run_sum[r][threadIdx.x % 16];
+    for (int r = 0; r < part; ++r) before += part_sum[r][threadIdx.x % 16];
     for (int c = first; c < end; ++c) {
         const long long at = static_cast<long long>(c) * experts + e;
         const int v = counts[at];
         counts[at] = before;
         before += v;
     }
-    if (run == 63) totals[e] = before;
+    if (part == 63) totals[e] = before;
 }
 
-__global__ __launch_bounds__(kChunkWaves * kWave) void plan_place_kernel(const int32_t* __restrict__ chosen, int entries, int experts, int bits,
-                                                                         const int* __restrict__ counts, const int* __restrict__ totals,
-                                                                         int32_t* __restrict__ offsets, int32_t* __restrict__ rows, int32_t* __restrict__ slots) {
+// totals == nullptr: counts are the runs' own, and this run adds them up.
+__global__ __launch_bounds__(kRunWaves * kWave) void plan_place_kernel(const int32_t* __restrict__ chosen, int entries, int experts, int bits, int run,
+                                                                       const int* __restrict__ counts, const int* __restrict__ totals, int runs,
+                                                                       int32_t* __restrict__ offsets, int32_t* __restrict__ rows, int32_t* __restrict__ slots) {
     extern __shared__ int plan_lds[];
-    int* start = plan_lds + kChunkWaves * experts;  // [expert + 1]
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    for (int e = threadIdx.x; e < experts; e += blockDim.x) start[e] = totals[e];
-    __syncthreads();
+    int *count = plan_lds, *start = plan_lds + kRunWaves * experts;  // [wave][expert], [expert + 1]
+    const int first = blockIdx.x * run, end = min(first + run, entries), per = per_wave(run);
+    // Entries of an expert in the runs before, kept in a register across the scan (an expert is one thread's).
+    int before = 0;
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {  // one trip: at most 1024 experts
+        int total = 0;
+        if (totals != nullptr) {
+            before = counts[static_cast<long long>(blockIdx.x) * experts + e];
+            total = totals[e];
+        } else {
+            for (int r = 0; r < runs; ++r) {
+                const int c = counts[static_cast<long long>(r) * experts + e];
+                before += r < static_cast<int>(blockIdx.x) ? c : 0;
+                total += c;
+            }
+        }
+        start[e] = total;
+    }
+    count_run(chosen, first, end, per, experts, count);
     scan_experts(start, experts);
+    const int total = start[experts];
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e <= experts; e += blockDim.x) offsets[e] = start[e];
-    const int chunk = blockIdx.x * kChunkWaves + wave;
-    const long long first = static_cast<long long>(chunk) * kChunk;
-    if (first >= entries) return;
-    const int end = static_cast<int>(first + kChunk < entries ? first + kChunk : entries);
-    int* next = plan_lds + wave * experts;  // this wavefront's own: no barrier needed
-    for (int e = lane; e < experts; e += kWave) next[e] = start[e] + counts[static_cast<long long>(chunk) * experts + e];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (int i = static_cast<int>(first) + lane; i < end; i += kWave)
-        if (i >= start[experts]) rows[i] = -1;
-    place_chunk(chosen, static_cast<int>(first), end, experts, bits, next, rows, slots);
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) start[e] += before;
+    __syncthreads();
+    place_run(chosen, first, end, per, experts, bits, count, start, total, rows, slots);
 }
 
 int bits_of(int experts) {
@@ -319,96 +441,167 @@ int check_route(const char* who, long long tokens, int experts, int k) {
     return 0;
 }
 
-}  // namespace
+// Runs of a plan: shorter ones where the longest would leave CUs without one.
+int run_entries(long long entries) { return entries >= 256ll * kRun ? kRun : kShortRun; }
+long long plan_runs(long long entries, int run) { return entries > 0 ? ceil_div(entries, static_cast<long long>(run)) : 1; }
+// One workgroup does it all: its counters fit 64 KiB of LDS.
+bool one_run(long long entries, int experts) { return entries <= kRun && experts <= 512; }
+size_t run_lds(int experts) { return (static_cast<size_t>(kRunWaves + 1) * experts + 1) * sizeof(int); }
 
-size_t expert_plan_workspace_bytes(long long tokens, int k, int experts) {
-    const long long entries = tokens * k;
-    if (tokens < 0 || k < 1 || experts < 1 || one_workgroup(entries, experts)) return 16;
-    return static_cast<size_t>((entries > 0 ? ceil_div(entries, static_cast<long long>(kChunk)) : 1) + 1) * experts * sizeof(int);
+// The plan behind the counts of its runs.
+int place_runs(const int32_t* chosen, int entries, int experts, int run, long long runs, int* counts, int32_t* offsets, int32_t* rows, int32_t* slots,
+               hipStream_t s) {
+    int* totals = nullptr;
+    if (runs > kSelfSum) {
+        totals = counts + runs * experts;
+        plan_sum_kernel<<<dim3(static_cast<unsigned>(ceil_div(experts, 16))), dim3(1024), 0, s>>>(counts, static_cast<int>(runs), experts, totals);
+        if (int rc = check_launch("plan_sum_kernel")) return rc;
+    }
+    const size_t lds = run_lds(experts);
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(plan_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+        if (e != hipSuccess) return hip_fail(e, "hipFuncSetAttribute(plan_place_kernel)");
+    }
+    plan_place_kernel<<<dim3(static_cast<unsigned>(runs)), dim3(kRunWaves * kWave), lds, s>>>(chosen, entries, experts, bits_of(experts), run, counts, totals,
+                                                                                             static_cast<int>(runs), offsets, rows, slots);
+    return check_launch("plan_place_kernel");
 }
 
-int launch_expert_plan(const int32_t* chosen, long long tokens, int k, int experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* ws,
-                       size_t ws_bytes, hipStream_t s) {
-    const char* who = "prism_expert_plan";
+int check_plan(const char* who, const int32_t* chosen, long long tokens, int k, int experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* ws,
+               size_t ws_bytes) {
     if (tokens < 0) return fail(1, "%s: negative number of tokens", who);
     if (experts < 1 || experts > kMaxExperts) return fail(1, "%s: %d experts, 1 to %d are supported", who, experts, kMaxExperts);
     if (k < 1) return fail(1, "%s: k=%d, at least 1 expert per token is needed", who, k);
     if (tokens > 0x7fffffffll || tokens * k > 0x7fffffffll - 4096) return fail(1, "%s: %lld tokens x %d: beyond 31 bits", who, tokens, k);
-    const int entries = static_cast<int>(tokens * k);
     if (offsets == nullptr || !aligned4(offsets)) return fail(1, "%s: offsets must be a 4-byte aligned device pointer", who);
-    if (entries > 0 && (chosen == nullptr || rows == nullptr || slots == nullptr || !aligned4(chosen) || !aligned4(rows) || !aligned4(slots)))
+    if (tokens > 0 && (chosen == nullptr || rows == nullptr || slots == nullptr || !aligned4(chosen) || !aligned4(rows) || !aligned4(slots)))
         return fail(1, "%s: experts, rows and slots must be 4-byte aligned device pointers", who);
-    const int bits = bits_of(experts);
-    if (one_workgroup(entries, experts)) {
-        const size_t lds = (static_cast<size_t>(kSmallWaves + 1) * experts + 1) * sizeof(int);
-        plan_small_kernel<<<dim3(1), dim3(kSmallWaves * kWave), lds, s>>>(chosen, entries, experts, bits, offsets, rows, slots);
-        return check_launch("plan_small_kernel");
-    }
-    if (ws == nullptr || !aligned4(ws) || ws_bytes < expert_plan_workspace_bytes(tokens, k, experts))
-        return fail(1, "%s: workspace of %zu bytes, %zu needed", who, ws == nullptr ? size_t{0} : ws_bytes, expert_plan_workspace_bytes(tokens, k, experts));
-    const int chunks = entries > 0 ? ceil_div(entries, kChunk) : 1;
-    int* counts = static_cast<int*>(ws);
-    int* totals = counts + static_cast<size_t>(chunks) * experts;
-    const dim3 grid(static_cast<unsigned>(ceil_div(chunks, kChunkWaves)));
-    const size_t lds = static_cast<size_t>(kChunkWaves) * experts * sizeof(int);
-    plan_count_kernel<<<grid, dim3(kChunkWaves * kWave), lds, s>>>(chosen, entries, experts, counts);
-    if (int rc = check_launch("plan_count_kernel")) return rc;
-    plan_sum_kernel<<<dim3(static_cast<unsigned>(ceil_div(experts, 16))), dim3(1024), 0, s>>>(counts, chunks, experts, totals);
-    if (int rc = check_launch("plan_sum_kernel")) return rc;
-    plan_place_kernel<<<grid, dim3(kChunkWaves * kWave), lds + (static_cast<size_t>(experts) + 1) * sizeof(int), s>>>(chosen, entries, experts, bits, counts, totals,
-                                                                                                                     offsets, rows, slots);
-    return check_launch("plan_place_kernel");
+    const size_t need = expert_plan_workspace_bytes(tokens, k, experts);
+    if (!one_run(tokens * k, experts) && (ws == nullptr || !aligned4(ws) || ws_bytes < need))
+        return fail(1, "%s: workspace of %zu bytes, %zu needed", who, ws == nullptr ? size_t{0} : ws_bytes, need);
+    return 0;
 }
 
-int launch_route_topk(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
-                      hipStream_t s) {
-    const char* who = "prism_route_topk";
+// The router's kernels for a logit type, a number of experts and an alignment: f(T, values of a lane, values of an access).
+template <typename F>
+int with_logits(int type, const void* logits, long long ld, int experts, F&& f) {
+    auto sized = [&](auto t, auto wide) {
+        using T = decltype(t);
+        using std::integral_constant;
+        constexpr int WIDE = decltype(wide)::value;
+        const bool packed = aligned16(logits) && ld % WIDE == 0 && experts % WIDE == 0;
+        auto go = [&](auto values) {
+            if (packed) return f(T{}, values, integral_constant<int, WIDE>{});
+            return f(T{}, values, integral_constant<int, 1>{});
+        };
+        if (experts <= 128) return go(integral_constant<int, 8>{});
+        if (experts <= 256) return go(integral_constant<int, 16>{});
+        return go(integral_constant<int, 64>{});
+    };
+    return type == kTypeF32 ? sized(float{}, std::integral_constant<int, 4>{}) : sized(uint16_t{}, std::integral_constant<int, 8>{});
+}
+
+}  // namespace
+
+// Room for the shortest runs: those of the router's 64 tokens, or of kShortRun entries.
+size_t expert_plan_workspace_bytes(long long tokens, int k, int experts) {
+    if (tokens < 0 || k < 1 || experts < 1 || one_run(tokens * k, experts)) return 16;
+    const long long by_entries = plan_runs(tokens * k, run_entries(tokens * k)), by_tokens = ceil_div(tokens, 64ll);
+    return static_cast<size_t>((by_entries > by_tokens ? by_entries : by_tokens) + 1) * experts * sizeof(int);
+}
+
+int launch_expert_plan(const int32_t* chosen, long long tokens, int k, int experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* ws,
+                       size_t ws_bytes, hipStream_t s) {
+    if (int rc = check_plan("prism_expert_plan", chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes)) return rc;
+    const int entries = static_cast<int>(tokens * k);
+    if (one_run(entries, experts)) {
+        plan_small_kernel<<<dim3(1), dim3(kRunWaves * kWave), run_lds(experts), s>>>(chosen, entries, experts, bits_of(experts), offsets, rows, slots);
+        return check_launch("plan_small_kernel");
+    }
+    const int run = run_entries(entries);
+    const long long runs = plan_runs(entries, run);
+    int* counts = static_cast<int*>(ws);
+    plan_count_kernel<<<dim3(static_cast<unsigned>(runs)), dim3(kRunWaves * kWave), static_cast<size_t>(experts) * sizeof(int), s>>>(chosen, entries, experts, run, counts);
+    if (int rc = check_launch("plan_count_kernel")) return rc;
+    return place_runs(chosen, entries, experts, run, runs, counts, offsets, rows, slots, s);
+}
+
+int check_route_call(const char* who, int type, const void* logits, long long ld, long long tokens, int experts, int k, const float* weights,
+                     const int32_t* chosen) {
     if (type != kTypeF32 && type != kTypeBf16) return fail(1, "%s: unknown logit type %d", who, type);
     if (int rc = check_route(who, tokens, experts, k)) return rc;
     if (tokens == 0) return 0;
     if (logits == nullptr || weights == nullptr || chosen == nullptr) return fail(1, "%s: null pointer", who);
     if (reinterpret_cast<uintptr_t>(logits) % (type == kTypeF32 ? 4 : 2) != 0 || !aligned4(weights) || !aligned4(chosen)) return fail(1, "%s: misaligned pointer", who);
     if (tokens > 1 && ld < experts) return fail(1, "%s: a row stride (%lld) is shorter than its row (%d)", who, ld, experts);
-    auto go = [&](auto t, auto lanes, auto values) {
+    return 0;
+}
+
+int launch_route_topk(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
+                      hipStream_t s) {
+    if (int rc = check_route_call("prism_route_topk", type, logits, ld, tokens, experts, k, weights, chosen)) return rc;
+    if (tokens == 0) return 0;
+    return with_logits(type, logits, ld, experts, [&](auto t, auto values, auto pack) {
         using T = decltype(t);
-        constexpr int L = decltype(lanes)::value, V = decltype(values)::value;
-        const unsigned blocks = static_cast<unsigned>(ceil_div(tokens, static_cast<long long>(kRouteBlock / L)));
-        route_topk_kernel<T, L, V><<<dim3(blocks), dim3(kRouteBlock), 0, s>>>(static_cast<const T*>(logits), ld, static_cast<int>(tokens), experts, k, renormalise,
+        constexpr int V = decltype(values)::value, P = decltype(pack)::value;
+        const unsigned blocks = static_cast<unsigned>(ceil_div(tokens, static_cast<long long>(kRouteBlock / kLanes)));
+        route_topk_kernel<T, V, P><<<dim3(blocks), dim3(kRouteBlock), 0, s>>>(static_cast<const T*>(logits), ld, static_cast<int>(tokens), experts, k, renormalise,
                                                                              weights, chosen);
         return check_launch("route_topk_kernel");
-    };
-    auto sized = [&](auto t) {
-        using std::integral_constant;
-        if (experts <= 64) return go(t, integral_constant<int, 16>{}, integral_constant<int, 4>{});
-        if (experts <= 128) return go(t, integral_constant<int, 16>{}, integral_constant<int, 8>{});
-        if (experts <= 256) return go(t, integral_constant<int, 16>{}, integral_constant<int, 16>{});
-        if (experts <= 512) return go(t, integral_constant<int, 64>{}, integral_constant<int, 8>{});
-        return go(t, integral_constant<int, 64>{}, integral_constant<int, 16>{});
-    };
-    return type == kTypeF32 ? sized(float{}) : sized(uint16_t{});
+    });
+}
+
+int launch_route_plan(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
+                      int32_t* offsets, int32_t* rows, int32_t* slots, void* ws, size_t ws_bytes, hipStream_t s) {
+    const char* who = "prism_route_plan";
+    if (int rc = check_route_call(who, type, logits, ld, tokens, experts, k, weights, chosen)) return rc;
+    if (int rc = check_plan(who, chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes)) return rc;
+    if (tokens == 0) return launch_expert_plan(chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes, s);
+    constexpr int TOKENS = kRunWaves * kWave / kLanes;  // of a workgroup
+    if (tokens > TOKENS && one_run(tokens * k, experts)) {  // too many for one workgroup's router, and no workspace to count in
+        if (int rc = launch_route_topk(type, logits, ld, tokens, experts, k, renormalise, weights, chosen, s)) return rc;
+        return launch_expert_plan(chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes, s);
+    }
+    const long long runs = ceil_div(tokens, static_cast<long long>(TOKENS));
+    const bool small = one_run(tokens * k, experts);  // else check_plan has seen to the workspace
+    const int rc = with_logits(type, logits, ld, experts, [&](auto t, auto values, auto pack) {
+        using T = decltype(t);
+        constexpr int V = decltype(values)::value, P = decltype(pack)::value;
+        const T* z = static_cast<const T*>(logits);
+        if (small)
+            route_small_kernel<T, V, P><<<dim3(1), dim3(kRunWaves * kWave), run_lds(experts), s>>>(z, ld, static_cast<int>(tokens), experts, k, renormalise, weights,
+                                                                                                  chosen, bits_of(experts), offsets, rows, slots);
+        else
+            route_count_kernel<T, V, P><<<dim3(static_cast<unsigned>(runs)), dim3(kRunWaves * kWave), static_cast<size_t>(experts) * sizeof(int), s>>>(
+                z, ld, static_cast<int>(tokens), experts, k, renormalise, weights, chosen, static_cast<int*>(ws));
+        return check_launch("route_small_kernel or route_count_kernel");
+    });
+    if (rc != 0 || small) return rc;
+    return place_runs(chosen, static_cast<int>(tokens * k), experts, TOKENS * k, runs, static_cast<int*>(ws), offsets, rows, slots, s);
 }
 
 int launch_route_backward(int type, const float* grad, const void* logits, long long ld, const float* weights, const int32_t* chosen, long long tokens,
                           int experts, int k, int renormalise, void* out, long long ldo, hipStream_t s) {
     const char* who = "prism_route_topk_backward";
-    if (type != kTypeF32 && type != kTypeBf16) return fail(1, "%s: unknown logit type %d", who, type);
-    if (int rc = check_route(who, tokens, experts, k)) return rc;
+    if (int rc = check_route_call(who, type, logits, ld, tokens, experts, k, weights, chosen)) return rc;
     if (tokens == 0) return 0;
-    if (grad == nullptr || logits == nullptr || weights == nullptr || chosen == nullptr || out == nullptr) return fail(1, "%s: null pointer", who);
+    if (grad == nullptr || out == nullptr) return fail(1, "%s: null pointer", who);
     const unsigned size = type == kTypeF32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(logits) % size != 0 || reinterpret_cast<uintptr_t>(out) % size != 0 || !aligned4(weights) || !aligned4(chosen) || !aligned4(grad))
-        return fail(1, "%s: misaligned pointer", who);
-    if (tokens > 1 && (ld < experts || ldo < experts)) return fail(1, "%s: a row stride is shorter than its row (%d)", who, experts);
+    if (reinterpret_cast<uintptr_t>(out) % size != 0 || !aligned4(grad)) return fail(1, "%s: misaligned pointer", who);
+    if (tokens > 1 && ldo < experts) return fail(1, "%s: a row stride is shorter than its row (%d)", who, experts);
     const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(out);
     if (a < b + ((tokens - 1) * ldo + experts) * size && b < a + ((tokens - 1) * ld + experts) * size) return fail(1, "%s: the result overlaps the logits", who);
-    const dim3 grid(static_cast<unsigned>(ceil_div(tokens, static_cast<long long>(kRouteBlock / 16))));
-    if (type == kTypeF32)
-        route_backward_kernel<float><<<grid, dim3(kRouteBlock), 0, s>>>(grad, static_cast<const float*>(logits), ld, weights, chosen, static_cast<int>(tokens), experts, k,
-                                                                        renormalise, static_cast<float*>(out), ldo);
-    else
-        route_backward_kernel<uint16_t><<<grid, dim3(kRouteBlock), 0, s>>>(grad, static_cast<const uint16_t*>(logits), ld, weights, chosen, static_cast<int>(tokens), experts,
-                                                                           k, renormalise, static_cast<uint16_t*>(out), ldo);
-    return check_launch("route_backward_kernel");
+    const dim3 grid(static_cast<unsigned>(ceil_div(tokens, static_cast<long long>(kRouteBlock / kLanes))));
+    auto go = [&](auto t, auto pack) {
+        using T = decltype(t);
+        route_backward_kernel<T, decltype(pack)::value><<<grid, dim3(kRouteBlock), 0, s>>>(grad, static_cast<const T*>(logits), ld, weights, chosen,
+                                                                                          static_cast<int>(tokens), experts, k, renormalise, static_cast<T*>(out), ldo);
+        return check_launch("route_backward_kernel");
+    };
+    const int wide = 16 / static_cast<int>(size);
+    const bool packed = aligned16(logits) && aligned16(out) && ld % wide == 0 && ldo % wide == 0 && experts % wide == 0;
+    if (type == kTypeF32) return packed ? go(float{}, std::integral_constant<int, 4>{}) : go(float{}, std::integral_constant<int, 1>{});
+    return packed ? go(uint16_t{}, std::integral_constant<int, 8>{}) : go(uint16_t{}, std::integral_constant<int, 1>{});
 }
 
 }  // namespace prism

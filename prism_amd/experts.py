@@ -125,22 +125,31 @@ def route_topk(logits: "torch.Tensor", k: int, renormalise: bool = True, out: Op
     chosen logits (renormalise) or over all of them. The plan is expert_plan's. out: a Routing (or five tensors in its
     order) to write into.
     """
-    if logits.dim() != 2:
-        raise ValueError("route_topk: logits must be [tokens, experts]")
     ld = _matrix(logits, _TYPES, "logits")
     T, E = logits.shape
     if out is None:
-        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=logits.device)  # noqa: E731
         k = int(k)
-        out = Routing(torch.empty((T, max(k, 0)), dtype=torch.float32, device=logits.device), new(T, max(k, 0)), new(E + 1), new(T * max(k, 0)), new(T, max(k, 0)))
+        new = lambda *shape: torch.empty([max(n, 0) for n in shape], dtype=torch.int32, device=logits.device)  # noqa: E731
+        out = Routing(torch.empty((T, max(k, 0)), dtype=torch.float32, device=logits.device), new(T, k), new(E + 1), new(T * k), new(T, k))
     else:
         out = Routing(*out)
         _whole(out.weights, torch.float32, "weights", T, k)
         _whole(out.experts, torch.int32, "experts", T, k)
-    _call("prism_route_topk", "route_topk", (logits, *out), logits.data_ptr(), _TYPES[logits.dtype], ld, T, E, k, bool(renormalise), out.weights.data_ptr(),
-          out.experts.data_ptr())
-    expert_plan(out.experts, E, out=out[2:])
+        _whole(out.offsets, torch.int32, "offsets", E + 1)
+        _whole(out.rows, torch.int32, "rows", T * k)
+        _whole(out.slots, torch.int32, "slots", T, k)
+    need, workspace = _plan_workspace(T, k, E, logits)
+    _call("prism_route_plan", "route_topk", (logits, *out), logits.data_ptr(), _TYPES[logits.dtype], ld, T, E, k, bool(renormalise), out.weights.data_ptr(),
+          out.experts.data_ptr(), out.offsets.data_ptr(), out.rows.data_ptr(), out.slots.data_ptr(), 0 if workspace is None else workspace.data_ptr(), need)
     return out
+
+
+def _plan_workspace(T: int, k: int, E: int, like: "torch.Tensor"):
+    """Bytes of a plan's workspace, and one (none where the plan is small enough to do without)."""
+    if T * k <= 4096 and E <= 512:
+        return 0, None
+    need = _lib.load().prism_expert_plan_workspace_bytes(T, k, E)
+    return need, torch.empty(need, dtype=torch.uint8, device=like.device) if need > 16 else None
 
 
 def expert_plan(experts: "torch.Tensor", num_experts: int, out=None) -> Tuple["torch.Tensor", "torch.Tensor", "torch.Tensor"]:
@@ -158,8 +167,7 @@ def expert_plan(experts: "torch.Tensor", num_experts: int, out=None) -> Tuple["t
     _whole(offsets, torch.int32, "offsets", num_experts + 1)
     _whole(rows, torch.int32, "rows", T * k)
     _whole(slots, torch.int32, "slots", T, k)
-    need = _lib.load().prism_expert_plan_workspace_bytes(T, k, num_experts)
-    workspace = torch.empty(need, dtype=torch.uint8, device=experts.device) if need > 16 else None
+    need, workspace = _plan_workspace(T, k, num_experts, experts)
     _call("prism_expert_plan", "expert_plan", (experts, offsets, rows, slots), experts.data_ptr(), T, k, num_experts, offsets.data_ptr(), rows.data_ptr(),
           slots.data_ptr(), workspace.data_ptr() if workspace is not None else 0, need)
     return offsets, rows, slots
