@@ -54,6 +54,7 @@ struct GroupedProblem {
     int depth;            // extent of c (forms with whole groups along c: unused)
     int out_rows;         // rows of one group's OUT (those forms only)
     int tiles_n;          // column tiles
+    bool near;            // rows of a tile within 32-bit offsets of each other
 };
 
 constexpr int kBK = 64;
@@ -127,45 +128,56 @@ __device__ __forceinline__ u32x4 load_packet(const uint16_t* at, int there) {
     return r;
 }
 
-template <int LINES, bool TURNED, int WAVES, bool ALIGNED>
-__device__ __forceinline__ void load_operand(uint16_t* tile, const OperandSource& src, int c0, int wave, int lane) {
+// A stage of an operand by direct-to-LDS loads. Bases and rows may lie anywhere (16 B loads take 2-byte aligned addresses),
+// but a chunk must be whole or absent, and the range check works on dwords: the depth is a multiple of 8 or the stage lies
+// inside it, and (turned) the lines are a multiple of 8 or the stage is not the last. A stage beyond the depth: zeros.
+template <int LINES, bool TURNED, int WAVES>
+__device__ __forceinline__ void load_direct(uint16_t* tile, const OperandSource& src, int c0, int wave, int lane) {
     using T = OperandTile<LINES, TURNED, WAVES>;
-    // Rows and row elements in memory that exist from the tile's corner on.
+    // Rows in memory that exist from the tile's corner on; those beyond the last are beyond the descriptor's extent (at most
+    // LINES or 65 rows of it: below 2 GiB by the launcher). Beyond the lines of a row of a turned operand lies the next row's
+    // head, which only enters lines that are not written; the extent ends with the lines of the stage's last row, or of the
+    // row behind it where there is one.
     const uint16_t* corner = src.base + (TURNED ? static_cast<long long>(c0) * src.ld : static_cast<long long>(c0));
-    const int rows = TURNED ? src.depth - c0 : src.lines;
-    const int elems = TURNED ? src.lines : src.depth - c0;
-    if constexpr (ALIGNED) {
-        // Lines, depth and rows are multiples of 8 elements along memory, so a chunk is whole or absent; rows beyond
-        // the last are beyond the descriptor's extent (at most LINES or 64 rows of it: below 2 GiB by the launcher).
-        const int in_tile = rows < T::ROWS ? (rows > 0 ? rows : 0) : T::ROWS;
-        const i32x4 rsrc = buffer_descriptor(corner, static_cast<uint32_t>(in_tile * src.ld * 2));
+    const int c_left = src.depth - c0, lines = src.lines < LINES ? src.lines : LINES;
+    const int elems = TURNED ? lines : c_left;
+    const int rows = TURNED ? (c_left < kBK + 1 ? c_left : kBK + 1) : lines;
+    uint32_t extent = TURNED ? static_cast<uint32_t>((rows - 1) * src.ld + lines) * 2u : static_cast<uint32_t>(rows * src.ld * 2);
+    if (c_left <= 0) extent = 0;
+    const i32x4 rsrc = buffer_descriptor(corner, extent);
 #pragma unroll
-        for (int p = 0; p < T::PASSES; ++p) {
-            const int chunk = T::chunk_of(p, wave, lane);
-            const uint32_t off = chunk * 8 < elems ? static_cast<uint32_t>((T::row_of(p, wave, lane) * src.ld + chunk * 8) * 2) : kBeyondExtent;
-            direct_load16_buffer(rsrc, off, 0u, &tile[T::lds_elem(p, wave)]);
-        }
-    } else {
+    for (int p = 0; p < T::PASSES; ++p) {
+        const int chunk = T::chunk_of(p, wave, lane);
+        const uint32_t at = static_cast<uint32_t>((T::row_of(p, wave, lane) * src.ld + chunk * 8) * 2);
+        direct_load16_buffer(rsrc, TURNED || chunk * 8 < elems ? at : kBeyondExtent, 0u, &tile[T::lds_elem(p, wave)]);
+    }
+}
+
+// The same by ordinary loads, for any stage of any operand.
+template <int LINES, bool TURNED, int WAVES>
+__device__ __forceinline__ void load_packets(uint16_t* tile, const OperandSource& src, int c0, int wave, int lane) {
+    using T = OperandTile<LINES, TURNED, WAVES>;
+    const uint16_t* corner = src.base + (TURNED ? static_cast<long long>(c0) * src.ld : static_cast<long long>(c0));
+    const int rows = TURNED ? src.depth - c0 : src.lines, elems = TURNED ? src.lines : src.depth - c0;
 #pragma unroll
-        for (int p = 0; p < T::PASSES; ++p) {
-            const int row = T::row_of(p, wave, lane), chunk = T::chunk_of(p, wave, lane);
-            const int there = row < rows ? elems - chunk * 8 : 0;
-            const u32x4 v = load_packet(corner + (there > 0 ? row * src.ld + chunk * 8 : 0), there);
-            *reinterpret_cast<u32x4*>(&tile[T::lds_elem(p, wave) + lane * 8]) = v;
-        }
+    for (int p = 0; p < T::PASSES; ++p) {
+        const int row = T::row_of(p, wave, lane), chunk = T::chunk_of(p, wave, lane);
+        const int there = row < rows ? elems - chunk * 8 : 0;
+        const u32x4 v = load_packet(corner + (there > 0 ? row * src.ld + chunk * 8 : 0), there);
+        *reinterpret_cast<u32x4*>(&tile[T::lds_elem(p, wave) + lane * 8]) = v;
     }
 }
 
 // ------------------------------------------------------------------------------------------- the general kernel --
 // 128 x 128 tiles, four waves of 64 x 64, one tile a workgroup: operands of any alignment, and problems with too few big
 // tiles for the chip. RAGGED_C: the groups lie along c (grad_b).
-// ALIGNED: direct-to-LDS loads into a ring of four stages of 64 c, three stages ahead; with at most one workgroup to a CU
-// nothing else hides the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of
-// the 0.3 its matrix instructions and LDS reads take). Else two stages, through registers.
+// Direct-to-LDS loads into a ring of four stages of 64 c, three stages ahead: with one workgroup to a CU nothing else hides
+// the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of 0.45). Not ALIGNED: the
+// last stage, or every one of rows too far apart for 32-bit offsets, comes by ordinary loads.
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, bool ALIGNED, typename OutT>
 __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
     constexpr int BM = 128, BN = 128, WAVES = 4, WM = BM / 2, WN = BN / 2, MI = WM / 16, NI = WN / 16;
-    constexpr int STAGES = ALIGNED ? 4 : 2;
+    constexpr int STAGES = 4;
     using PT = OperandTile<BM, P_TURNED, WAVES>;
     using QT = OperandTile<BN, Q_TURNED, WAVES>;
     constexpr int LOADS = PT::PASSES + QT::PASSES;  // of a wave and stage
@@ -199,8 +211,16 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
     f32x4 acc[MI][NI] = {};
     const int tiles = __builtin_amdgcn_readfirstlane(ps.depth > 0 ? (ps.depth + kBK - 1) / kBK : 1);  // without depth: a stage of zeros
     auto load = [&](int t) {  // beyond the last: zeros, so that every stage has its loads in flight
-        load_operand<BM, P_TURNED, WAVES, ALIGNED>(Ps[t % STAGES], ps, t * kBK, wave, lane);
-        load_operand<BN, Q_TURNED, WAVES, ALIGNED>(Qs[t % STAGES], qs, t * kBK, wave, lane);
+        uint16_t *to_p = Ps[t % STAGES], *to_q = Qs[t % STAGES];
+        // By ordinary loads, the stages before have landed as well when this one has (loads are waited for in order), and the
+        // counting in front of the barriers, which takes every stage's direct loads to be under way, errs to the safe side.
+        if (!ALIGNED && t < tiles && (t == tiles - 1 || !g.near)) {
+            load_packets<BM, P_TURNED, WAVES>(to_p, ps, t * kBK, wave, lane);
+            load_packets<BN, Q_TURNED, WAVES>(to_q, qs, t * kBK, wave, lane);
+        } else {
+            load_direct<BM, P_TURNED, WAVES>(to_p, ps, t * kBK, wave, lane);
+            load_direct<BN, Q_TURNED, WAVES>(to_q, qs, t * kBK, wave, lane);
+        }
     };
     auto barrier = [&](auto in_flight) {  // of this wave's loads at most so many are still on their way
         asm volatile("" ::: "memory");    // the compiler knows neither the loads' writes to LDS nor what the barrier orders
@@ -223,28 +243,16 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
                 for (int j = 0; j < NI; ++j) mfma_in_place(acc[i][j], fq[j], fp[i]);
         }
     };
-    using none = std::integral_constant<int, 0>;
-    if constexpr (ALIGNED) {
-        // The barrier in front of stage t: it has landed, and everybody is done with stage t - 1, whose place t + 3 takes.
+    // The barrier in front of stage t: it has landed, and everybody is done with stage t - 1, whose place t + 3 takes.
 #pragma unroll
-        for (int t = 0; t < STAGES - 1; ++t) load(t);
-        int t = 0;
-        do {
-            barrier(std::integral_constant<int, (STAGES - 2) * LOADS>{});
-            load(t + STAGES - 1);
-            multiply(t);
-        } while (++t < tiles);
-        __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));  // the loads beyond the last stage write LDS
-    } else {
-        load(0);
-        barrier(none{});
-        int t = 0;
-        do {
-            if (t + 1 < tiles) load(t + 1);
-            multiply(t);
-            barrier(none{});
-        } while (++t < tiles);
-    }
+    for (int t = 0; t < STAGES - 1; ++t) load(t);
+    int t = 0;
+    do {
+        barrier(std::integral_constant<int, (STAGES - 2) * LOADS>{});
+        load(t + STAGES - 1);
+        multiply(t);
+    } while (++t < tiles);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));  // the loads beyond the last stage write LDS
     grouped_settle();
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -894,12 +902,12 @@ Kernel choose_kernel(const GroupedProblem& g, bool can_few, bool can_big) {
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
 int run(GroupedProblem g, const char* who, hipStream_t s) {
     constexpr bool FORWARD = !P_TURNED && !Q_TURNED;
-    // Direct-to-LDS loads need 16 B chunks that are whole or absent (bases, strides and the extents along memory in
-    // multiples of 8 elements) and 32-bit offsets inside a tile. What is not aligned runs on the general kernel, or on the
-    // one for few rows, which reads B where it lies.
+    // Aligned: 16 B chunks are whole or absent throughout (bases, strides and the extents along memory in multiples of 8
+    // elements), with 32-bit offsets inside a tile. What is not runs on the general kernel, or on the one for few rows.
+    g.near = g.ldp < (1 << 21) && g.ldq < (1 << 21);
     const int p_along = P_TURNED ? g.out_rows : g.depth, q_along = Q_TURNED ? g.cols : g.depth;
     const bool aligned = aligned16(g.P) && aligned16(g.Q) && g.ldp % 8 == 0 && g.ldq % 8 == 0 && (RAGGED_C || g.group_stride % 8 == 0) &&
-                         p_along % 8 == 0 && q_along % 8 == 0 && g.ldp < (1 << 21) && g.ldq < (1 << 21);
+                         p_along % 8 == 0 && q_along % 8 == 0 && g.near;
     const Kernel kernel = choose_kernel<RAGGED_C>(g, FORWARD, aligned && g.groups <= kBigGroups && cu_count() >= 8);
     if constexpr (FORWARD)
         if (kernel == Kernel::kFew) return run_few<OutT>(g, who, s);
