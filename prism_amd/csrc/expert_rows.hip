@@ -17,44 +17,71 @@ namespace {
 
 constexpr int kRowsBlock = 256, kRowsWaves = kRowsBlock / kWave;
 
-// A lane's packet: BYTES of consecutive elements, as fp32 values and back.
-template <typename T, int BYTES>
-struct Packet {
-    static constexpr int N = BYTES / static_cast<int>(sizeof(T));
-    T raw[N];
-    static __device__ __forceinline__ Packet load(const T* p) {
-        Packet r;
-        __builtin_memcpy(r.raw, __builtin_assume_aligned(p, BYTES), BYTES);
-        return r;
-    }
-    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(__builtin_assume_aligned(p, BYTES), raw, BYTES); }
-};
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(uint16_t v) { return __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16); }
 __device__ __forceinline__ void from_float(float& to, float v) { to = v; }
 __device__ __forceinline__ void from_float(uint16_t& to, float v) { to = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }  // nearest even
 
+// A lane's packet: 16 B of consecutive elements of a row, at any element (16 B accesses need no more alignment than that;
+// as packets of 4 B, rows of 4100 B ran at half the bandwidth), the last of a row cut to what is there. ONCE: non-temporal,
+// for rows that no other wavefront touches: stores always (8192 tokens x 8 x 4096 bf16, gather: 172 -> 139 us), loads where
+// there is more of them than the memory-side cache holds (backward of the sum: 219 -> 204 us; 32 MB of them: 8.1 -> 12.5).
+template <typename T>
+struct Packet {
+    static constexpr int N = 16 / static_cast<int>(sizeof(T));
+    typedef T Vector __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    T v[N];
+    template <bool ONCE>
+    static __device__ __forceinline__ Packet load(const T* p, int there) {
+        Packet r;
+        if (there >= N) {
+            const Vector* at = reinterpret_cast<const Vector*>(p);
+            const Vector raw = ONCE ? __builtin_nontemporal_load(at) : *at;
+#pragma unroll
+            for (int i = 0; i < N; ++i) r.v[i] = raw[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r.v[i] = i < there ? p[i] : T{};
+        }
+        return r;
+    }
+    template <bool ONCE>
+    __device__ __forceinline__ void store(T* p, int there) const {
+        if (there >= N) {
+            Vector raw;
+#pragma unroll
+            for (int i = 0; i < N; ++i) raw[i] = v[i];
+            if constexpr (ONCE) __builtin_nontemporal_store(raw, reinterpret_cast<Vector*>(p));
+            else *reinterpret_cast<Vector*>(p) = raw;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < there) p[i] = v[i];
+        }
+    }
+};
+
 // One wavefront per 64 packets of a slot's row.
-template <typename T, int BYTES>
+template <typename T>
 __global__ __launch_bounds__(kRowsBlock) void expert_gather_kernel(const T* __restrict__ x, long long ldx, int tokens, int k,
                                                                    const int32_t* __restrict__ rows, T* __restrict__ out, long long ldo,
                                                                    int n_slots, int width, int parts) {
-    using P = Packet<T, BYTES>;
+    using P = Packet<T>;
     const long long unit = static_cast<long long>(blockIdx.x) * kRowsWaves + threadIdx.x / kWave;
     const int slot = static_cast<int>(unit / parts);
     const int at = (static_cast<int>(unit % parts) * kWave + threadIdx.x % kWave) * P::N;
     if (slot >= n_slots || at >= width) return;
     const int row = rows[slot], token = row / k;
     if (row < 0 || token >= tokens) return;
-    P::load(x + token * ldx + at).store(out + slot * ldo + at);
+    P::template load<false>(x + token * ldx + at, width - at).template store<true>(out + slot * ldo + at, width - at);
 }
 
 // One wavefront per 64 packets of a token's row; U rows in flight.
-template <typename T, int BYTES, bool WEIGHTED>
+template <typename T, bool WEIGHTED, bool STREAM>
 __global__ __launch_bounds__(kRowsBlock) void expert_sum_kernel(const T* __restrict__ y, long long ldy, int n_slots,
                                                                 const float* __restrict__ weights, const int32_t* __restrict__ slots, int k,
                                                                 T* __restrict__ out, long long ldo, int tokens, int width, int parts) {
-    using P = Packet<T, BYTES>;
+    using P = Packet<T>;
     constexpr int U = 4;
     const long long unit = static_cast<long long>(blockIdx.x) * kRowsWaves + threadIdx.x / kWave;
     const int token = static_cast<int>(unit / parts);
@@ -70,29 +97,27 @@ __global__ __launch_bounds__(kRowsBlock) void expert_sum_kernel(const T* __restr
             const int slot = j < k ? slots[static_cast<long long>(token) * k + j] : -1;
             const bool there = slot >= 0 && slot < n_slots;
             w[u] = there ? (WEIGHTED ? weights[static_cast<long long>(token) * k + j] : 1.0f) : 0.0f;
-            if (there) v[u] = P::load(y + slot * ldy + at);
-            else
-#pragma unroll
-                for (int i = 0; i < P::N; ++i) v[u].raw[i] = T{};
+            v[u] = P::template load<STREAM>(y + (there ? slot * ldy + at : 0), there ? width - at : 0);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < P::N; ++i) sum[i] = __builtin_fmaf(w[u], as_float(v[u].raw[i]), sum[i]);
+            for (int i = 0; i < P::N; ++i) sum[i] = __builtin_fmaf(w[u], as_float(v[u].v[i]), sum[i]);
     }
     P r;
 #pragma unroll
-    for (int i = 0; i < P::N; ++i) from_float(r.raw[i], sum[i]);
-    r.store(out + token * ldo + at);
+    for (int i = 0; i < P::N; ++i) from_float(r.v[i], sum[i]);
+    r.template store<false>(out + token * ldo + at, width - at);
 }
 
-// One wavefront per (token, j): its slot's row of dy, and the dot product of its row of y.
-template <typename T, int BYTES>
+// One wavefront per (token, j): its slot's row of dy, and the dot product of its row of y. The wavefronts of a token follow
+// each other: dout's row is in the caches for all but the first.
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kRowsBlock) void expert_sum_backward_kernel(const T* __restrict__ dout, long long ldd, const T* __restrict__ y,
                                                                          long long ldy, const float* __restrict__ weights,
                                                                          const int32_t* __restrict__ slots, int n_slots, T* __restrict__ dy,
                                                                          long long lddy, float* __restrict__ dw, long long entries, int k, int width) {
-    using P = Packet<T, BYTES>;
+    using P = Packet<T>;
     const int lane = threadIdx.x % kWave;
     const long long entry = static_cast<long long>(blockIdx.x) * kRowsWaves + threadIdx.x / kWave;
     if (entry >= entries) return;
@@ -101,15 +126,16 @@ __global__ __launch_bounds__(kRowsBlock) void expert_sum_backward_kernel(const T
     if (slot >= 0 && slot < n_slots) {
         const float w = weights[entry];
         const T* up = dout + entry / k * ldd;
+#pragma unroll 2
         for (int at = lane * P::N; at < width; at += kWave * P::N) {
-            const P a = P::load(up + at), b = P::load(y + slot * ldy + at);
+            const P a = P::template load<false>(up + at, width - at), b = P::template load<STREAM>(y + slot * ldy + at, width - at);
             P r;
 #pragma unroll
             for (int i = 0; i < P::N; ++i) {
-                dot = __builtin_fmaf(as_float(a.raw[i]), as_float(b.raw[i]), dot);
-                from_float(r.raw[i], w * as_float(a.raw[i]));
+                dot = __builtin_fmaf(as_float(a.v[i]), as_float(b.v[i]), dot);
+                from_float(r.v[i], w * as_float(a.v[i]));
             }
-            r.store(dy + slot * lddy + at);
+            r.template store<true>(dy + slot * lddy + at, width - at);
         }
     }
 #pragma unroll
@@ -117,28 +143,11 @@ __global__ __launch_bounds__(kRowsBlock) void expert_sum_backward_kernel(const T
     if (lane == 0) dw[entry] = dot;
 }
 
-// The widest packet that every row start, and the row length, is a multiple of.
-int packet_bytes(int size, long long width, std::initializer_list<const void*> bases, std::initializer_list<long long> strides) {
-    uintptr_t all = static_cast<uintptr_t>(width) * size;
-    for (const void* b : bases) all |= reinterpret_cast<uintptr_t>(b);
-    for (long long s : strides) all |= static_cast<uintptr_t>(s) * size;
-    for (int bytes = 16; bytes > size; bytes /= 2)
-        if (all % bytes == 0) return bytes;
-    return size;
-}
+// More than the 256 MiB memory-side cache would keep of the rows.
+bool streams(long long rows, long long width, int size) { return rows * width * size > (192ll << 20); }
 
 template <typename F>
-int with_packet(int type, int bytes, F&& f) {
-    if (type == kTypeF32) {
-        if (bytes == 16) return f(float{}, std::integral_constant<int, 16>{});
-        if (bytes == 8) return f(float{}, std::integral_constant<int, 8>{});
-        return f(float{}, std::integral_constant<int, 4>{});
-    }
-    if (bytes == 16) return f(uint16_t{}, std::integral_constant<int, 16>{});
-    if (bytes == 8) return f(uint16_t{}, std::integral_constant<int, 8>{});
-    if (bytes == 4) return f(uint16_t{}, std::integral_constant<int, 4>{});
-    return f(uint16_t{}, std::integral_constant<int, 2>{});
-}
+int with_type(int type, F&& f) { return type == kTypeF32 ? f(float{}) : f(uint16_t{}); }
 
 int check_rows(const char* who, int type, long long tokens, int k, long long n_slots, long long width, std::initializer_list<const void*> bases,
                std::initializer_list<long long> strides) {
@@ -172,12 +181,12 @@ int launch_expert_gather(int type, const void* x, long long ldx, long long token
     if (rows == nullptr || !aligned4(rows)) return fail(1, "%s: rows must be a 4-byte aligned device pointer", who);
     const int size = type == kTypeF32 ? 4 : 2;
     if (rows_overlap(x, tokens, ldx, out, n_slots, ldo, width, size)) return fail(1, "%s: x and the result overlap", who);
-    return with_packet(type, packet_bytes(size, width, {x, out}, {ldx, ldo}), [&](auto t, auto bytes) {
+    return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T, bytes>::N)));
+        const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T>::N)));
         const long long blocks = ceil_div(n_slots * parts, static_cast<long long>(kRowsWaves));
         if (blocks > 0x7fffffffll) return fail(1, "%s: too much work for one launch", who);
-        expert_gather_kernel<T, bytes><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
+        expert_gather_kernel<T><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
             static_cast<const T*>(x), ldx, static_cast<int>(tokens), k, rows, static_cast<T*>(out), ldo, static_cast<int>(n_slots), static_cast<int>(width), parts);
         return check_launch("expert_gather_kernel");
     });
@@ -192,18 +201,19 @@ int launch_expert_sum(int type, const void* y, long long ldy, long long n_slots,
     if (out == nullptr || ldo < width) return fail(1, "%s: null result or a row stride shorter than its row", who);
     const int size = type == kTypeF32 ? 4 : 2;
     if (rows_overlap(y, n_slots, ldy, out, tokens, ldo, width, size)) return fail(1, "%s: y and the result overlap", who);
-    return with_packet(type, packet_bytes(size, width, {y, out}, {ldy, ldo}), [&](auto t, auto bytes) {
+    return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T, bytes>::N)));
+        const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T>::N)));
         const long long blocks = ceil_div(tokens * parts, static_cast<long long>(kRowsWaves));
         if (blocks > 0x7fffffffll) return fail(1, "%s: too much work for one launch", who);
-        auto go = [&](auto weighted) {
-            expert_sum_kernel<T, bytes, weighted><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
+        auto go = [&](auto weighted, auto stream) {
+            expert_sum_kernel<T, weighted, stream><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
                 static_cast<const T*>(y), ldy, static_cast<int>(n_slots), weights, slots, k, static_cast<T*>(out), ldo, static_cast<int>(tokens),
                 static_cast<int>(width), parts);
         };
-        if (weights != nullptr) go(std::true_type{});
-        else go(std::false_type{});
+        const bool stream = streams(n_slots, width, size);
+        if (weights != nullptr) stream ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+        else stream ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
         return check_launch("expert_sum_kernel");
     });
 }
@@ -219,11 +229,15 @@ int launch_expert_sum_backward(int type, const void* dout, long long ldd, const 
     if (rows_overlap(y, n_slots, ldy, dy, n_slots, lddy, width, size) || rows_overlap(dout, tokens, ldd, dy, n_slots, lddy, width, size))
         return fail(1, "%s: the gradient of y overlaps an input", who);
     const long long entries = tokens * k;
-    return with_packet(type, packet_bytes(size, width, {dout, y, dy}, {ldd, ldy, lddy}), [&](auto t, auto bytes) {
+    return with_type(type, [&](auto t) {
         using T = decltype(t);
-        expert_sum_backward_kernel<T, bytes><<<dim3(static_cast<unsigned>(ceil_div(entries, static_cast<long long>(kRowsWaves)))), dim3(kRowsBlock), 0, s>>>(
-            static_cast<const T*>(dout), ldd, static_cast<const T*>(y), ldy, weights, slots, static_cast<int>(n_slots), static_cast<T*>(dy), lddy, dw, entries, k,
-            static_cast<int>(width));
+        auto go = [&](auto stream) {
+            expert_sum_backward_kernel<T, stream><<<dim3(static_cast<unsigned>(ceil_div(entries, static_cast<long long>(kRowsWaves)))), dim3(kRowsBlock), 0, s>>>(
+                static_cast<const T*>(dout), ldd, static_cast<const T*>(y), ldy, weights, slots, static_cast<int>(n_slots), static_cast<T*>(dy), lddy, dw, entries, k,
+                static_cast<int>(width));
+        };
+        if (streams(n_slots, width, size)) go(std::true_type{});
+        else go(std::false_type{});
         return check_launch("expert_sum_backward_kernel");
     });
 }
