@@ -51,7 +51,7 @@ def _call(function: str, name: str, tensors, *args) -> None:
                 raise ValueError(f"{name}: expected a tensor in device memory (cuda), got a host tensor")
             raise ValueError(f"{name}: tensors on different devices ({tensors[0].device}, {t.device})")
     launch = getattr(_lib._lib or _lib.load(), function)
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         rc = launch(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -107,12 +107,13 @@ def _groups(t: "torch.Tensor", dtypes, name: str, n: Optional[int] = None, k: Op
     return ld, stride
 
 
-def _out(out: Optional["torch.Tensor"], shape, dtype, like: "torch.Tensor") -> "torch.Tensor":
+def _out(out: Optional["torch.Tensor"], name: str, n: int, m: int, dtype, dtypes, like: "torch.Tensor") -> Tuple["torch.Tensor", int]:
+    """The caller's row-major result, checked, or a new one; and the elements between its rows."""
     if out is not None:
-        return out
+        return out, _matrix(out, dtypes, name, n, m)
     if dtype not in _TYPES:
         raise TypeError(f"out_dtype: {dtype} not in {tuple(_TYPES)}")
-    return torch.empty(shape, dtype=dtype, device=like.device)
+    return (like.new_empty((n, m)) if dtype == like.dtype else like.new_empty((n, m), dtype=dtype)), max(m, 1)
 
 
 # ------------------------------------------------------------------ router --
@@ -183,8 +184,7 @@ def route_topk_backward(grad_weights: "torch.Tensor", logits: "torch.Tensor", we
     _whole(grad_weights, torch.float32, "grad_weights", T, k)
     _whole(weights, torch.float32, "weights", T, k)
     _whole(experts, torch.int32, "experts", T, k)
-    out = _out(out, (T, E), logits.dtype, logits)
-    ldo = _matrix(out, (logits.dtype,), "out", T, E)
+    out, ldo = _out(out, "out", T, E, logits.dtype, (logits.dtype,), logits)
     _call("prism_route_topk_backward", "route_topk_backward", (logits, grad_weights, weights, experts, out), grad_weights.data_ptr(), logits.data_ptr(),
           _TYPES[logits.dtype], ld, weights.data_ptr(), experts.data_ptr(), T, E, k, bool(renormalise), out.data_ptr(), ldo)
     return out
@@ -200,8 +200,7 @@ def expert_gather(x: "torch.Tensor", rows: "torch.Tensor", k: int, out: Optional
     if rows.dim() != 1:
         raise ValueError("expert_gather: rows must be one-dimensional")
     _whole(rows, torch.int32, "rows", rows.shape[0])
-    out = _out(out, (rows.shape[0], H), x.dtype, x)
-    ldo = _matrix(out, (x.dtype,), "out", rows.shape[0], H)
+    out, ldo = _out(out, "out", rows.shape[0], H, x.dtype, (x.dtype,), x)
     _call("prism_expert_gather", "expert_gather", (x, rows, out), x.data_ptr(), _TYPES[x.dtype], ldx, T, k, rows.data_ptr(), out.data_ptr(), ldo,
           rows.shape[0], H)
     return out
@@ -216,8 +215,7 @@ def _sum(name: str, y: "torch.Tensor", weights: Optional["torch.Tensor"], slots:
     _whole(slots, torch.int32, "slots", T, k)
     if weights is not None:
         _whole(weights, torch.float32, "weights", T, k)
-    out = _out(out, (T, H), y.dtype, y)
-    ldo = _matrix(out, (y.dtype,), "out", T, H)
+    out, ldo = _out(out, "out", T, H, y.dtype, (y.dtype,), y)
     _call("prism_expert_combine", name, (y, slots, out) if weights is None else (y, weights, slots, out), y.data_ptr(), _TYPES[y.dtype], ldy, R,
           0 if weights is None else weights.data_ptr(), slots.data_ptr(), T, k, out.data_ptr(), ldo, H)
     return out
@@ -248,10 +246,11 @@ def expert_combine_backward(grad_out: "torch.Tensor", y: "torch.Tensor", weights
     _whole(slots, torch.int32, "slots", T, k)
     _whole(weights, torch.float32, "weights", T, k)
     ldd = _matrix(grad_out, (y.dtype,), "grad_out", T, H)
-    grad_y = _out(grad_y, (R, H), y.dtype, y)
-    lddy = _matrix(grad_y, (y.dtype,), "grad_y", R, H)
-    grad_weights = _out(grad_weights, (T, k), torch.float32, y)
-    _whole(grad_weights, torch.float32, "grad_weights", T, k)
+    grad_y, lddy = _out(grad_y, "grad_y", R, H, y.dtype, (y.dtype,), y)
+    if grad_weights is None:
+        grad_weights = torch.empty_like(weights)
+    else:
+        _whole(grad_weights, torch.float32, "grad_weights", T, k)
     _call("prism_expert_combine_backward", "expert_combine_backward", (y, grad_out, weights, slots, grad_y, grad_weights), grad_out.data_ptr(),
           _TYPES[y.dtype], ldd, y.data_ptr(), ldy, weights.data_ptr(), slots.data_ptr(), T, k, grad_y.data_ptr(), lddy, grad_weights.data_ptr(), R, H)
     return grad_y, grad_weights
@@ -275,8 +274,7 @@ def gemm_bf16_grouped(A: "torch.Tensor", B: "torch.Tensor", offsets: "torch.Tens
     ldb, stride = _groups(B, _BF16, "B", None, K)
     G, N, _ = B.shape
     _whole(offsets, torch.int32, "offsets", G + 1)
-    D = _out(D, (R, N), out_dtype, A)
-    ldd = _matrix(D, _TYPES, "D", R, N)
+    D, ldd = _out(D, "D", R, N, out_dtype, _TYPES, A)
     _call("prism_gemm_bf16_grouped", "gemm_bf16_grouped", (A, B, offsets, D), G, R, N, K, A.data_ptr(), lda, B.data_ptr(), ldb, stride,
           offsets.data_ptr(), D.data_ptr(), ldd, _TYPES[D.dtype])
     return D
@@ -290,8 +288,7 @@ def gemm_bf16_grouped_grad_a(dD: "torch.Tensor", B: "torch.Tensor", offsets: "to
     ldb, stride = _groups(B, _BF16, "B", N, None)
     G, _, K = B.shape
     _whole(offsets, torch.int32, "offsets", G + 1)
-    dA = _out(dA, (R, K), out_dtype, dD)
-    lda = _matrix(dA, _TYPES, "dA", R, K)
+    dA, lda = _out(dA, "dA", R, K, out_dtype, _TYPES, dD)
     _call("prism_gemm_bf16_grouped_grad_a", "gemm_bf16_grouped_grad_a", (dD, B, offsets, dA), G, R, N, K, dD.data_ptr(), ldd, B.data_ptr(), ldb, stride,
           offsets.data_ptr(), dA.data_ptr(), lda, _TYPES[dA.dtype])
     return dA
@@ -309,7 +306,10 @@ def gemm_bf16_grouped_grad_b(dD: "torch.Tensor", A: "torch.Tensor", offsets: "to
         raise ValueError("offsets: expected groups + 1 entries")
     G = offsets.shape[0] - 1
     _whole(offsets, torch.int32, "offsets", G + 1)
-    dB = _out(dB, (G, N, K), out_dtype, dD)
+    if dB is None:
+        if out_dtype not in _TYPES:
+            raise TypeError(f"out_dtype: {out_dtype} not in {tuple(_TYPES)}")
+        dB = dD.new_empty((G, N, K), dtype=out_dtype)
     ldb, stride = _groups(dB, _TYPES, "dB", N, K)
     if dB.shape[0] != G:
         raise ValueError(f"dB: {dB.shape[0]} matrices for {G} groups")
@@ -350,8 +350,7 @@ def gemv_w4(x: "torch.Tensor", q: "torch.Tensor", scales: "torch.Tensor", group_
         _whole(offsets, torch.int32, "offsets", G + 1)
     elif G != 1:
         raise ValueError(f"gemv_w4: {G} weight matrices need offsets")
-    out = _out(out, (R, N), out_dtype, x)
-    ldo = _matrix(out, _TYPES, "out", R, N)
+    out, ldo = _out(out, "out", R, N, out_dtype, _TYPES, x)
     _call("prism_gemv_w4", "gemv_w4", [t for t in (x, q, scales, zeros, offsets, out) if t is not None], G, R, N, K, x.data_ptr(), ldx, q.data_ptr(), ldq,
           stride, scales.data_ptr(), zeros.data_ptr() if zeros is not None else 0, group_size, offsets.data_ptr() if offsets is not None else 0, out.data_ptr(),
           ldo, _TYPES[out.dtype])
