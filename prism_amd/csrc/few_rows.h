@@ -27,7 +27,7 @@ __device__ __forceinline__ void instruction_x(const bf16x8 (&x)[LOADS], bf16x8& 
     }
 }
 
-// How a column tile's K is shared: by as few wavefronts as give every CU eight of them (each has a fixed cost, and their
+// How a column tile's K is shared: by as few wavefronts as give every CU per_cu of them (each has a fixed cost, and their
 // parts meet at the end), not more than there are steps of step_k. `busy`: the row tiles that exist, about.
 inline int few_rows_k_parts(long long busy, int N, int K, int step_k, int most, int per_cu) {
     int parts = 1;

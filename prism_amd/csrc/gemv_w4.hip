@@ -237,8 +237,8 @@ __device__ __forceinline__ f32x4 multiply_slice(const W4Slice& p) {
     return total;
 }
 
-// Eight wavefronts for up to 16 rows: 8 / k_parts column tiles of 16, each by k_parts wavefronts that take consecutive
-// steps (a slice each).
+// Up to 16 rows by n_parts column tiles of 16, each by k_parts wavefronts (two to eight in all) that take consecutive steps,
+// a slice each.
 template <StepScales SCALES, bool ZEROS, typename OutT>
 __global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Problem p) {
     __shared__ f32x4 parts[kW4Waves * kWave];
@@ -342,7 +342,11 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
     const long long row_tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16) : ceil_div(rows, 16ll);
     // Of a group table's tiles about as many exist as there are rows or groups.
     const long long busy = offsets != nullptr ? (rows < groups ? rows : row_tiles) : row_tiles;
-    p.k_parts = few_rows_k_parts(busy, N, K, kW4Block, kW4Waves, 8);
+    // Twelve wavefronts a CU, none with less than a round of few rows (512 k: shorter slices only have the loop's last,
+    // unpipelined part). Against eight and single steps: 16384 x 16384 by 1 row 35.6 -> 30.2 us, 8192 x 1024 by 16 rows 7.1 -> 5.3,
+    // 2048 x 1024 by 4 rows 5.0 -> 3.7, none of sixteen sizes slower by 1 %; sixteen wavefronts gain 7 % on 64 matrices of
+    // 1536 x 2048 by 32 rows but lose 40 % on 14336 x 4096 by 1 row (9.1 -> 13.0 us) and 19 % on 8 of 2048 x 2048 by 64.
+    p.k_parts = few_rows_k_parts(busy, N, K, 4 * kW4Block, kW4Waves, 12);
     p.n_parts = p.k_parts < kW4Few ? kW4Few / p.k_parts : 1;
     p.tiles_n = ceil_div(N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;
