@@ -171,13 +171,13 @@ __device__ __forceinline__ void load_packets(uint16_t* tile, const OperandSource
 // ------------------------------------------------------------------------------------------- the general kernel --
 // 128 x 128 tiles, four waves of 64 x 64, one tile a workgroup: operands of any alignment, and problems with too few big
 // tiles for the chip. RAGGED_C: the groups lie along c (grad_b).
-// Direct-to-LDS loads into a ring of four stages of 64 c, three stages ahead: with one workgroup to a CU nothing else hides
-// the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of 0.45). Not ALIGNED: the
-// last stage, or every one of rows too far apart for 32-bit offsets, comes by ordinary loads.
-template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, bool ALIGNED, typename OutT>
+// Direct-to-LDS loads into a ring of STAGES stages of 64 c. Four, three ahead, where there is a tile to a CU and nothing else
+// hides the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of 0.45); two where
+// there are more tiles and two workgroups share a CU (choose_kernel). Not ALIGNED: the last stage, or every one of rows too
+// far apart for 32-bit offsets, comes by ordinary loads.
+template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, bool ALIGNED, int STAGES, typename OutT>
 __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
     constexpr int BM = 128, BN = 128, WAVES = 4, WM = BM / 2, WN = BN / 2, MI = WM / 16, NI = WN / 16;
-    constexpr int STAGES = 4;
     using PT = OperandTile<BM, P_TURNED, WAVES>;
     using QT = OperandTile<BN, Q_TURNED, WAVES>;
     constexpr int LOADS = PT::PASSES + QT::PASSES;  // of a wave and stage
@@ -874,12 +874,15 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
 // 32 or fewer groups; `used` groups have rows, which the host takes to be as many as there can be, and a group wastes half a
 // row tile):
 //   few      5 + B read once per 16-row tile at 5.3 TB/s with up to 4 rows a group, 3.9 with more (see instruction_x)
-//   general  rounds of 256 tiles of 128 x 128 at 4 + 0.48 a stage, or B once at 4.3 TB/s
+//   general  rounds of 256 tiles of 128 x 128 at 4 + 0.48 a stage with a ring of four stages, of 512 at 4 + 1.1 with one of
+//            two, or B once at 4.3 TB/s
 //   big      rounds of 256 tiles of 256 x 256 at 8 + 1.2 a stage (stages in pairs), or B once at 4.3 TB/s
 // Measured, few / general / big: 64 rows of 32 groups, 2048 x 2048: 56 / 57 / 65 us; 512 rows: 101 / 63 / 70; 2048 rows:
 // 252 / 67 / 73; 8192 rows: - / 106 / 82; 100 rows of 8 groups, 256 x 4096: 10 / 34 / 69; 2000 rows of 16, 768 x 768: 38 /
 // 12 / 21. Gradient of B, general / big: 512 rows of 32 groups, 2048 x 2048: 137 / 66; 1000 rows of 32, 304 x 512: 10 / 12.
-enum class Kernel { kFew, kGeneral, kBig };
+// General, four stages / two: 5003 rows of 24 groups, 1000 x 1048: 32.9 / 28.7; 4000 of 8, 2048 x 1024: 30.4 / 25.3; 2000 of 16,
+// 768 x 768: 12.2 / 13.4; 6000 of 16, 1536 x 2048: 79 / 83; gradient of B, 1000 rows of 32, 304 x 512: 10.0 / 7.8.
+enum class Kernel { kFew, kGeneral, kGeneralPairs, kBig };
 template <bool RAGGED_C>
 Kernel choose_kernel(const GroupedProblem& g, bool can_few, bool can_big) {
     const double rows = g.rows, groups = g.groups, used = rows < groups ? rows : groups;
@@ -887,16 +890,18 @@ Kernel choose_kernel(const GroupedProblem& g, bool can_few, bool can_big) {
     auto rounds = [](double tiles) { return static_cast<double>(static_cast<long long>((tiles + 255.0) / 256.0)); };
     const double depth = RAGGED_C ? rows / groups : static_cast<double>(g.depth), stages = static_cast<double>(static_cast<long long>((depth + 63) / 64));
     const double b_us = RAGGED_C ? 0.0 : used * g.cols * depth * 2 / 4.3e6;
-    auto tiled = [&](int edge, double fixed, double stage_us, double n_stages) {
+    auto tiled = [&](int edge, int per_cu, double fixed, double stage_us, double n_stages) {
         const double tiles = (RAGGED_C ? groups * ceil_div(g.out_rows, edge) : row_tiles(edge)) * ceil_div(g.cols, edge);
-        const double us = rounds(tiles) * (fixed + stage_us * n_stages);
+        const double us = rounds(tiles / per_cu) * (fixed + stage_us * n_stages);
         return 2 + (us > b_us ? us : b_us);
     };
-    const double general = tiled(128, 4, 0.48, stages > 1 ? stages : 1);
-    const double big = can_big ? tiled(256, 8, 1.2, stages > 2 ? stages + static_cast<long long>(stages) % 2 : 2) : 1e30;
+    const double single = tiled(128, 1, 4, 0.48, stages > 1 ? stages : 1), pairs = tiled(128, 2, 4, 1.1, stages > 1 ? stages : 1);
+    const double general = single <= pairs ? single : pairs;
+    const double big = can_big ? tiled(256, 1, 8, 1.2, stages > 2 ? stages + static_cast<long long>(stages) % 2 : 2) : 1e30;
     const double few = can_few ? 5 + row_tiles(16) * g.cols * depth * 2 / (rows <= 4 * groups ? 5.3e6 : 3.9e6) : 1e30;
     if (few <= general && few <= big) return Kernel::kFew;
-    return general <= big ? Kernel::kGeneral : Kernel::kBig;
+    if (big < general) return Kernel::kBig;
+    return single <= pairs ? Kernel::kGeneral : Kernel::kGeneralPairs;
 }
 
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
@@ -920,8 +925,13 @@ int run(GroupedProblem g, const char* who, hipStream_t s) {
         return check_launch("gemm_grouped_big_kernel");
     }
     const dim3 grid(static_cast<unsigned>(tiles_m * g.tiles_n));
-    if (aligned) gemm_grouped_kernel<P_TURNED, Q_TURNED, RAGGED_C, true, OutT><<<grid, dim3(256), 0, s>>>(g);
-    else gemm_grouped_kernel<P_TURNED, Q_TURNED, RAGGED_C, false, OutT><<<grid, dim3(256), 0, s>>>(g);
+    auto start = [&](auto stages) {
+        constexpr int STAGES = decltype(stages)::value;
+        if (aligned) gemm_grouped_kernel<P_TURNED, Q_TURNED, RAGGED_C, true, STAGES, OutT><<<grid, dim3(256), 0, s>>>(g);
+        else gemm_grouped_kernel<P_TURNED, Q_TURNED, RAGGED_C, false, STAGES, OutT><<<grid, dim3(256), 0, s>>>(g);
+    };
+    if (kernel == Kernel::kGeneralPairs) start(std::integral_constant<int, 2>{});
+    else start(std::integral_constant<int, 4>{});
     return check_launch("gemm_grouped_kernel");
 }
 

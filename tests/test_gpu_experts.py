@@ -104,6 +104,13 @@ def test_grouped_products_with_more_tiles_than_workgroups(prism, sizes, n, k):
     grouped_case(prism, sizes, n, k, torch.float32, seed=n + 1)
 
 
+@pytest.mark.parametrize("sizes,n,k,start,pad", [([257] * 9, 1301, 523, 1, 0), ([1] * 20 + [900, 0, 640], 1000, 1048, 0, 0), ([40] * 30, 305, 513, 3, 1), ([900, 800], 1160, 1096, 8, 8)],
+                         ids=lambda v: str(len(v)) if isinstance(v, list) else str(v))
+def test_grouped_products_of_two_workgroups_to_a_unit(prism, sizes, n, k, start, pad):
+    for dtype in TYPES:
+        grouped_case(prism, sizes, n, k, dtype, seed=n + k, first=2, behind=9, start=start, pad=pad)
+
+
 def test_grouped_products_many_groups(prism):
     rng = np.random.default_rng(4)
     grouped_case(prism, list(rng.integers(0, 4, 1000)), 64, 128, torch.float32, seed=9)
