@@ -35,6 +35,9 @@ inline int check_launch(const char* kernel) {
     return 0;
 }
 
+// A launch has fewer than 2^32 threads along x.
+inline bool launchable(long long blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }

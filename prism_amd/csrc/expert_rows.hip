@@ -185,7 +185,7 @@ int launch_expert_gather(int type, const void* x, long long ldx, long long token
         using T = decltype(t);
         const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T>::N)));
         const long long blocks = ceil_div(n_slots * parts, static_cast<long long>(kRowsWaves));
-        if (blocks > 0x7fffffffll) return fail(1, "%s: too much work for one launch", who);
+        if (!launchable(blocks, kRowsBlock)) return fail(1, "%s: too much work for one launch", who);
         expert_gather_kernel<T><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
             static_cast<const T*>(x), ldx, static_cast<int>(tokens), k, rows, static_cast<T*>(out), ldo, static_cast<int>(n_slots), static_cast<int>(width), parts);
         return check_launch("expert_gather_kernel");
@@ -205,7 +205,7 @@ int launch_expert_sum(int type, const void* y, long long ldy, long long n_slots,
         using T = decltype(t);
         const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T>::N)));
         const long long blocks = ceil_div(tokens * parts, static_cast<long long>(kRowsWaves));
-        if (blocks > 0x7fffffffll) return fail(1, "%s: too much work for one launch", who);
+        if (!launchable(blocks, kRowsBlock)) return fail(1, "%s: too much work for one launch", who);
         auto go = [&](auto weighted, auto stream) {
             expert_sum_kernel<T, weighted, stream><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
                 static_cast<const T*>(y), ldy, static_cast<int>(n_slots), weights, slots, k, static_cast<T*>(out), ldo, static_cast<int>(tokens),
@@ -229,6 +229,7 @@ int launch_expert_sum_backward(int type, const void* dout, long long ldd, const 
     if (rows_overlap(y, n_slots, ldy, dy, n_slots, lddy, width, size) || rows_overlap(dout, tokens, ldd, dy, n_slots, lddy, width, size))
         return fail(1, "%s: the gradient of y overlaps an input", who);
     const long long entries = tokens * k;
+    if (!launchable(ceil_div(entries, static_cast<long long>(kRowsWaves)), kRowsBlock)) return fail(1, "%s: too much work for one launch", who);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto stream) {

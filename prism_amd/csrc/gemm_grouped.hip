@@ -865,7 +865,7 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
     p.n_parts = p.k_parts < kFewLeast ? kFewLeast / p.k_parts : 1;
     p.tiles_n = ceil_div(p.N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;
-    if (blocks > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
+    if (!launchable(blocks, kFewWaves * kWave)) return fail(1, "%s: too many tiles", who);
     gemm_grouped_few_kernel<OutT><<<dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(p.k_parts * p.n_parts * kWave)), 0, s>>>(p);
     return check_launch("gemm_grouped_few_kernel");
 }
@@ -919,7 +919,7 @@ int run(GroupedProblem g, const char* who, hipStream_t s) {
     const int edge = kernel == Kernel::kBig ? 256 : 128;
     g.tiles_n = ceil_div(g.cols, edge);
     const long long tiles_m = RAGGED_C ? static_cast<long long>(g.groups) * ceil_div(g.out_rows, edge) : most_row_tiles(g.rows, g.groups, edge);
-    if (tiles_m * g.tiles_n > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
+    if (!launchable(tiles_m * g.tiles_n, 256)) return fail(1, "%s: too many tiles", who);
     if (kernel == Kernel::kBig) {
         gemm_grouped_big_kernel<P_TURNED, Q_TURNED, RAGGED_C, OutT><<<dim3(static_cast<unsigned>(cu_count() / 8 * 8)), dim3(256), 0, s>>>(g);
         return check_launch("gemm_grouped_big_kernel");
@@ -953,6 +953,8 @@ int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int
                       : form == GroupedForm::kGradA ? "prism_gemm_bf16_grouped_grad_a" : "prism_gemm_bf16_grouped_grad_b";
     if (groups < 0 || rows < 0 || N < 0 || K < 0) return fail(1, "%s: negative dimension (%d groups, %lld rows, N=%d, K=%d)", who, groups, rows, N, K);
     if (rows > 0x7fffffffll - 256) return fail(1, "%s: %lld rows, at most 2^31 - 257 are supported", who, rows);
+    if (groups > 0x7fffffff - 4096 || N > 0x7fffffff - 4096 || K > 0x7fffffff - 4096)
+        return fail(1, "%s: %d groups, N=%d, K=%d: at most 2^31 - 4097 are supported", who, groups, N, K);
     if (out_type != kTypeF32 && out_type != kTypeBf16) return fail(1, "%s: unknown output type %d", who, out_type);
     const int size = out_type == kTypeF32 ? 4 : 2;
     const bool grad_b = form == GroupedForm::kGradB;

@@ -317,7 +317,8 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
     if (out_type != kTypeF32 && out_type != kTypeBf16) return fail(1, "%s: unknown output type %d", who, out_type);
     if (group_size < 32 || group_size % 32 != 0) return fail(1, "%s: group size %d, multiples of 32 are supported", who, group_size);
     if (rows > 0x7fffffffll - 256) return fail(1, "%s: %lld rows, at most 2^31 - 257 are supported", who, rows);
-    if (K > 0x7fffffff - 4096) return fail(1, "%s: K=%d is too large", who, K);
+    if (groups > 0x7fffffff - 4096 || N > 0x7fffffff - 4096 || K > 0x7fffffff - 4096)
+        return fail(1, "%s: %d groups, N=%d, K=%d: at most 2^31 - 4097 are supported", who, groups, N, K);
     if (offsets == nullptr && groups > 1) return fail(1, "%s: %d weight matrices need offsets", who, groups);
     if (groups == 0 || rows == 0 || N == 0) return 0;
     if (ldx < K || ldy < N || ldq < (static_cast<long long>(K) + 1) / 2) return fail(1, "%s: a row stride is shorter than its row", who);
@@ -350,7 +351,7 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
     p.n_parts = p.k_parts < kW4Few ? kW4Few / p.k_parts : 1;
     p.tiles_n = ceil_div(N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;
-    if (blocks > 0x7fffffffll) return fail(1, "%s: too many tiles", who);
+    if (!launchable(blocks, kW4Waves * kWave)) return fail(1, "%s: too many tiles", who);
     p.row_tiles = static_cast<int>(row_tiles);
     const dim3 grid(static_cast<unsigned>(blocks));
     if (group_size == 128) return go<StepScales::kOne>(p, out_type, grid, s);

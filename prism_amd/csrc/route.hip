@@ -437,7 +437,8 @@ int check_route(const char* who, long long tokens, int experts, int k) {
     if (tokens < 0) return fail(1, "%s: negative number of tokens", who);
     if (experts < 1 || experts > kMaxExperts) return fail(1, "%s: %d experts, 1 to %d are supported", who, experts, kMaxExperts);
     if (k < 1 || k > kMaxChosen || k > experts) return fail(1, "%s: k=%d, 1 to %d and at most the number of experts (%d) are supported", who, k, kMaxChosen, experts);
-    if (tokens * k > 0x7fffffffll - 4096) return fail(1, "%s: %lld tokens x %d: beyond 31 bits", who, tokens, k);
+    if (tokens > 0x7fffffffll || tokens * k > 0x7fffffffll - 4096) return fail(1, "%s: %lld tokens x %d: beyond 31 bits", who, tokens, k);
+    if (!launchable(ceil_div(tokens, 64ll), 64 * kLanes)) return fail(1, "%s: %lld tokens are too much work for one launch", who, tokens);
     return 0;
 }
 
@@ -505,7 +506,7 @@ int with_logits(int type, const void* logits, long long ld, int experts, F&& f) 
 
 // Room for the shortest runs: those of the router's 64 tokens, or of kShortRun entries.
 size_t expert_plan_workspace_bytes(long long tokens, int k, int experts) {
-    if (tokens < 0 || k < 1 || experts < 1 || one_run(tokens * k, experts)) return 16;
+    if (tokens < 0 || k < 1 || experts < 1 || experts > kMaxExperts || tokens > 0x7fffffffll || one_run(tokens * k, experts)) return 16;
     const long long by_entries = plan_runs(tokens * k, run_entries(tokens * k)), by_tokens = ceil_div(tokens, 64ll);
     return static_cast<size_t>((by_entries > by_tokens ? by_entries : by_tokens) + 1) * experts * sizeof(int);
 }

@@ -21,6 +21,7 @@ One layer, forward:
 """
 from __future__ import annotations
 
+from operator import index
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -60,6 +61,14 @@ def _call(function: str, name: str, tensors, *args) -> None:
         _check(rc, name)
 
 
+def _int(v, name: str) -> int:
+    """An int argument of the C functions, which would keep only its lower 32 bits."""
+    v = index(v)
+    if not -0x80000000 <= v <= 0x7fffffff:
+        raise ValueError(f"{name}: {v} is beyond 31 bits")
+    return v
+
+
 def _matrix(t: "torch.Tensor", dtypes, name: str, rows: Optional[int] = None, cols: Optional[int] = None) -> int:
     """Checks a row-major matrix; returns the elements between its rows."""
     if t.dtype not in dtypes:
@@ -68,6 +77,8 @@ def _matrix(t: "torch.Tensor", dtypes, name: str, rows: Optional[int] = None, co
     if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
         raise ValueError(f"{name}: shape {tuple(shape)}, expected ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
     n, m = shape
+    if m > 0x7fffffff:
+        raise ValueError(f"{name}: rows of {m} elements, beyond 31 bits")
     ld, one = t.stride()
     if one != 1 and m > 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
@@ -95,6 +106,8 @@ def _groups(t: "torch.Tensor", dtypes, name: str, n: Optional[int] = None, k: Op
     if t.dim() != 3 or (n is not None and t.shape[1] != n) or (k is not None and t.shape[2] != k):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected (groups, {'N' if n is None else n}, {'K' if k is None else k})")
     g, n, k = t.shape
+    if max(g, n, k) > 0x7fffffff:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, beyond 31 bits")
     if k > 1 and t.stride(2) != 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
     ld = t.stride(1) if n > 1 and k > 0 else max(k, 1)
@@ -128,10 +141,12 @@ def route_topk(logits: "torch.Tensor", k: int, renormalise: bool = True, out: Op
     """
     ld = _matrix(logits, _TYPES, "logits")
     T, E = logits.shape
+    k = _int(k, "k")
+    if not 1 <= k <= E or k > 32:  # before anything of this size is allocated
+        raise ValueError(f"route_topk: k={k}, 1 to 32 and at most the number of experts ({E}) are supported")
     if out is None:
-        k = int(k)
-        new = lambda *shape: torch.empty([max(n, 0) for n in shape], dtype=torch.int32, device=logits.device)  # noqa: E731
-        out = Routing(torch.empty((T, max(k, 0)), dtype=torch.float32, device=logits.device), new(T, k), new(E + 1), new(T * k), new(T, k))
+        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=logits.device)  # noqa: E731
+        out = Routing(torch.empty((T, k), dtype=torch.float32, device=logits.device), new(T, k), new(E + 1), new(T * k), new(T, k))
     else:
         out = Routing(*out)
         _whole(out.weights, torch.float32, "weights", T, k)
@@ -161,9 +176,12 @@ def expert_plan(experts: "torch.Tensor", num_experts: int, out=None) -> Tuple["t
         raise ValueError("expert_plan: experts must be [tokens, k]")
     T, k = experts.shape
     _whole(experts, torch.int32, "experts", T, k)
+    num_experts = _int(num_experts, "num_experts")
+    if not 1 <= num_experts <= 1024:
+        raise ValueError(f"expert_plan: {num_experts} experts, 1 to 1024 are supported")
     if out is None:
         new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=experts.device)  # noqa: E731
-        out = (new(max(int(num_experts), 0) + 1), new(T * k), new(T, k))
+        out = (new(num_experts + 1), new(T * k), new(T, k))
     offsets, rows, slots = out
     _whole(offsets, torch.int32, "offsets", num_experts + 1)
     _whole(rows, torch.int32, "rows", T * k)
@@ -197,6 +215,7 @@ def expert_gather(x: "torch.Tensor", rows: "torch.Tensor", k: int, out: Optional
     out: undefined). x: [T, H] fp32 or bf16; rows: [R] int32, as route_topk gives it."""
     ldx = _matrix(x, _TYPES, "x")
     T, H = x.shape
+    k = _int(k, "k")
     if rows.dim() != 1:
         raise ValueError("expert_gather: rows must be one-dimensional")
     _whole(rows, torch.int32, "rows", rows.shape[0])
@@ -331,7 +350,7 @@ def gemv_w4(x: "torch.Tensor", q: "torch.Tensor", scales: "torch.Tensor", group_
     """
     ldx = _matrix(x, _BF16, "x")
     R, K = x.shape
-    group_size = int(group_size)
+    group_size = _int(group_size, "group_size")
     if group_size < 1:
         raise ValueError(f"gemv_w4: group size {group_size}")
     if q.dim() == 2:

@@ -133,3 +133,40 @@ def test_python_mirror():
             (lambda: prism.gemv_w4(bf(1, 64), torch.zeros(2, 16, 32, dtype=torch.uint8), bf(2, 16, 2), 32), ValueError, "offsets")):
         with pytest.raises(error, match=text):
             call()
+
+
+def test_sizes_beyond_a_launch_or_31_bits(lib):
+    far = [P + (i << 44) for i in range(8)]
+    many = 1 << 28
+    refused(lib, lib.prism_expert_gather(far[0], 1, 8, 4, 2, far[1], far[2], 8, many, 8, None), "one launch")
+    refused(lib, lib.prism_expert_combine(far[0], 1, 8, 4, None, far[1], many, 2, far[2], 8, 8, None), "one launch")
+    refused(lib, lib.prism_expert_combine_backward(far[0], 1, 8, far[1], 8, far[2], far[3], many >> 2, 2, far[4], 8, far[5], 8, 8, None), "one launch")
+    for tokens in (many + 1, (1 << 62) + 1):
+        refused(lib, lib.prism_route_topk(far[0], 1, 8, tokens, 8, 1, 1, far[1], far[2], None), "one launch" if tokens < 1 << 31 else "31 bits")
+    refused(lib, lib.prism_route_topk_backward(far[0], far[1], 0, 8, far[2], far[3], many + 1, 8, 1, 0, far[4], 8, None), "one launch")
+    assert lib.prism_expert_plan_workspace_bytes(1 << 20, 8, 1 << 20) == 16  # experts that no call takes
+    top = 0x7fffffff
+    for name in ("prism_gemm_bf16_grouped", "prism_gemm_bf16_grouped_grad_a"):
+        refused(lib, getattr(lib, name)(1, 1, 1, top, far[0], top, far[1], top, top, far[2], far[3], top, 0, None), "at most")
+        refused(lib, getattr(lib, name)(1, 1, top, 1, far[0], top, far[1], 1, top, far[2], far[3], top, 0, None), "at most")
+        refused(lib, getattr(lib, name)(top, 1, 1, 1, far[0], 1, far[1], 1, 1, far[2], far[3], 1, 0, None), "at most")
+    refused(lib, lib.prism_gemm_bf16_grouped_grad_b(1, 1, top, 1, far[0], top, far[1], 1, far[2], far[3], 1, top, 0, None), "at most")
+    refused(lib, lib.prism_gemm_bf16_grouped(1 << 20, 1 << 20, 1 << 20, 8, far[0], 8, far[1], 8, 1 << 23, far[2], far[3], 1 << 20, 0, None), "too many tiles")
+    refused(lib, lib.prism_gemv_w4(1, 1, top, 32, far[0], 32, far[1], 16, 0, far[2], None, 32, None, far[3], top, 1, None), "at most")
+    refused(lib, lib.prism_gemv_w4(1, 1 << 20, 1 << 20, 32, far[0], 32, far[1], 16, 0, far[2], None, 32, None, far[3], 1 << 20, 1, None), "too many tiles")
+
+
+def test_python_integers_are_not_cut():
+    x, i32 = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(4, 2, dtype=torch.int32)
+    for call in (lambda: prism.route_topk(torch.zeros(4, 8), (1 << 32) + 1), lambda: prism.expert_plan(i32, (1 << 32) + 1),
+                 lambda: prism.expert_gather(x, i32.view(-1), (1 << 32) + 2),
+                 lambda: prism.gemv_w4(x, torch.zeros(16, 32, dtype=torch.uint8), torch.zeros(16, 1, dtype=torch.bfloat16), (1 << 32) + 32),
+                 lambda: prism.gemm_bf16_grouped(torch.empty(1, 1 << 31, dtype=torch.bfloat16, device="meta"), x.view(1, 4, 64), i32.view(-1)[:2])):
+        with pytest.raises(ValueError, match="31 bits"):
+            call()
+    for call in (lambda: prism.route_topk(torch.zeros(4, 8), 0), lambda: prism.route_topk(torch.zeros(4, 8), 9), lambda: prism.route_topk(torch.zeros(4, 64), 33),
+                 lambda: prism.expert_plan(i32, 0), lambda: prism.expert_plan(i32, 1025)):
+        with pytest.raises(ValueError, match="supported"):
+            call()
+    with pytest.raises(TypeError):
+        prism.expert_gather(x, i32.view(-1), 2.0)

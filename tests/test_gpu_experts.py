@@ -409,6 +409,52 @@ def test_row_moves_with_wrong_entries_stay_inside(prism):
     assert bool((grad_w.reshape(-1)[[1, 2, 3, 4]] == 0).all())
 
 
+def test_row_moves_and_router_beyond_32_bit_offsets(prism):
+    """Rows 2^30 + 8 elements apart: the last of four begins beyond 2^31 elements."""
+    far = (1 << 30) + 8
+
+    def spread(values):
+        view = torch.as_strided(torch.empty(3 * far + values.shape[1], dtype=values.dtype, device=DEV), tuple(values.shape), (far, 1))
+        view.copy_(values)
+        return view
+
+    x, y = normal(1, 4, 264).bfloat16(), normal(2, 4, 264).bfloat16()
+    rows = torch.tensor([3, 1, 0, 2], dtype=torch.int32, device=DEV)
+    slots = torch.tensor([[2], [1], [3], [0]], dtype=torch.int32, device=DEV)
+    w = normal(3, 4, 1)
+    out = spread(torch.zeros_like(x))
+    prism.expert_gather(spread(x), rows, 1, out)
+    assert torch.equal(out, x[rows.long()])
+    far_y, order = spread(y), slots[:, 0].long()
+    prism.expert_combine(far_y, w, slots, out)
+    near(out, y[order].double() * w.double(), (y[order].double() * w.double()).abs(), 2)
+    grad_y, grad_w = prism.expert_combine_backward(spread(x), far_y, w, slots, grad_y=out)
+    near(grad_w[:, 0], (x.double() * y[order].double()).sum(1), (x.double() * y[order].double()).abs().sum(1), 264 + 8)
+    near(grad_y[order], x.double() * w.double(), (x.double() * w.double()).abs(), 1)
+    logits = normal(4, 4, 64).bfloat16()
+    want, got = prism.route_topk(logits, 3), prism.route_topk(spread(logits), 3)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    up = normal(5, 4, 3)
+    grad = prism.route_topk_backward(up, spread(logits), got.weights, got.experts, renormalise=False, out=spread(torch.zeros_like(logits)))
+    assert torch.equal(grad, prism.route_topk_backward(up, logits, want.weights, want.experts, renormalise=False))
+
+
+def test_no_tokens_or_no_slots(prism):
+    none = lambda *s, dtype=torch.float32: torch.empty(s, dtype=dtype, device=DEV)  # noqa: E731
+    r = prism.route_topk(none(0, 8), 2)
+    assert r.weights.shape == (0, 2) and bool((r.offsets == 0).all())
+    assert prism.route_topk_backward(r.weights, none(0, 8), r.weights, r.experts).shape == (0, 8)
+    assert prism.expert_gather(none(0, 16), r.rows, 2).shape == (0, 16)
+    assert prism.expert_combine(none(0, 16), r.weights, r.slots).shape == (0, 16)
+    nowhere = torch.full((3, 2), -1, dtype=torch.int32, device=DEV)
+    assert bool((prism.expert_combine(none(0, 16), normal(1, 3, 2), nowhere) == 0).all())
+    grad_y, grad_w = prism.expert_combine_backward(normal(1, 3, 16), none(0, 16), normal(1, 3, 2), nowhere)
+    assert grad_y.shape == (0, 16) and bool((grad_w == 0).all())
+    y = prism.gemv_w4(none(3, 0, dtype=torch.bfloat16), none(5, 0, dtype=torch.uint8), none(5, 0, dtype=torch.bfloat16), 32)
+    assert y.shape == (3, 5) and bool((y == 0).all())
+    assert prism.gemv_w4(none(0, 64, dtype=torch.bfloat16), none(5, 32, dtype=torch.uint8), none(5, 2, dtype=torch.bfloat16), 32).shape == (0, 5)
+
+
 # ----------------------------------------------------------------------------------------------- together, as in use --
 
 def layer(prism, x, router, up, down, k):
