@@ -6,7 +6,8 @@
 // Unused slots are left as they are, a token without experts gets zeros. Sums run over j (and, in the dot products,
 // over the row) in 32 bits and in a fixed order: the same bits on every run.
 //
-// HBM-bound: every row is read once and written once.
+// HBM-bound: every row is read once and written once. 8192 tokens x 8 x 4096 bf16, a random choice of 64 experts: gather 139 us
+// (604 MB, 4.3 TB/s), sum 114 us (5.3 TB/s), its backward 219 us (1.14 GB, 5.2 TB/s).
 #include <initializer_list>
 #include <type_traits>
 
@@ -25,7 +26,7 @@ __device__ __forceinline__ void from_float(uint16_t& to, float v) { to = __built
 // A lane's packet: 16 B of consecutive elements of a row, at any element (16 B accesses need no more alignment than that;
 // as packets of 4 B, rows of 4100 B ran at half the bandwidth), the last of a row cut to what is there. ONCE: non-temporal,
 // for rows that no other wavefront touches: stores always (8192 tokens x 8 x 4096 bf16, gather: 172 -> 139 us), loads where
-// there is more of them than the memory-side cache holds (backward of the sum: 219 -> 204 us; 32 MB of them: 8.1 -> 12.5).
+// there is more of them than the memory-side cache holds (backward of the sum: 231 -> 219 us; 32 MB of them: 8.1 -> 12.5).
 template <typename T>
 struct Packet {
     static constexpr int N = 16 / static_cast<int>(sizeof(T));
@@ -110,24 +111,27 @@ __global__ __launch_bounds__(kRowsBlock) void expert_sum_kernel(const T* __restr
     r.template store<false>(out + token * ldo + at, width - at);
 }
 
-// One wavefront per (token, j): its slot's row of dy, and the dot product of its row of y. The wavefronts of a token follow
-// each other: dout's row is in the caches for all but the first.
+// One wavefront per (token, j), or two (STREAM): its slot's row of dy, and the dot product of its row of y. The wavefronts of
+// a token follow each other: dout's row is in the caches for all but the first. Where the rows come from and go to memory in
+// an order of no locality, two wavefronts a row keep half as many rows under way: 8192 tokens x 8 x 4096 bf16 235 -> 219 us
+// (5.2 TB/s; slots in the tokens' order: 188), x 2048 119 -> 112, 16384 x 2 x 7168 230 -> 233; where the caches hold a good part,
+// one is better (2048 x 4 x 4096: 24.6 against 26.3 us, 600 x 8 x 4096 fp32: 30 against 36).
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kRowsBlock) void expert_sum_backward_kernel(const T* __restrict__ dout, long long ldd, const T* __restrict__ y,
                                                                          long long ldy, const float* __restrict__ weights,
                                                                          const int32_t* __restrict__ slots, int n_slots, T* __restrict__ dy,
                                                                          long long lddy, float* __restrict__ dw, long long entries, int k, int width) {
     using P = Packet<T>;
-    const int lane = threadIdx.x % kWave;
-    const long long entry = static_cast<long long>(blockIdx.x) * kRowsWaves + threadIdx.x / kWave;
-    if (entry >= entries) return;
-    const int slot = slots[entry];
+    constexpr int SHARE = STREAM ? 2 : 1;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, part = wave % SHARE;
+    const long long entry = static_cast<long long>(blockIdx.x) * (kRowsWaves / SHARE) + wave / SHARE;
+    const int slot = entry < entries ? slots[entry] : -1;
     float dot = 0.0f;
     if (slot >= 0 && slot < n_slots) {
         const float w = weights[entry];
         const T* up = dout + entry / k * ldd;
 #pragma unroll 2
-        for (int at = lane * P::N; at < width; at += kWave * P::N) {
+        for (int at = (part * kWave + lane) * P::N; at < width; at += SHARE * kWave * P::N) {
             const P a = P::template load<false>(up + at, width - at), b = P::template load<STREAM>(y + slot * ldy + at, width - at);
             P r;
 #pragma unroll
@@ -140,7 +144,13 @@ __global__ __launch_bounds__(kRowsBlock) void expert_sum_backward_kernel(const T
     }
 #pragma unroll
     for (int d = kWave / 2; d > 0; d /= 2) dot += __shfl_xor(dot, d);
-    if (lane == 0) dw[entry] = dot;
+    if constexpr (SHARE == 2) {
+        __shared__ float behind[kRowsWaves];
+        if (lane == 0) behind[wave] = dot;
+        __syncthreads();
+        dot += behind[wave | 1];  // of the first wavefront; the second one's is not used
+    }
+    if (lane == 0 && part == 0 && entry < entries) dw[entry] = dot;
 }
 
 // More than the 256 MiB memory-side cache would keep of the rows.
@@ -229,16 +239,17 @@ int launch_expert_sum_backward(int type, const void* dout, long long ldd, const 
     if (rows_overlap(y, n_slots, ldy, dy, n_slots, lddy, width, size) || rows_overlap(dout, tokens, ldd, dy, n_slots, lddy, width, size))
         return fail(1, "%s: the gradient of y overlaps an input", who);
     const long long entries = tokens * k;
-    if (!launchable(ceil_div(entries, static_cast<long long>(kRowsWaves)), kRowsBlock)) return fail(1, "%s: too much work for one launch", who);
+    const bool stream = streams(n_slots, width, size);
+    const long long blocks = ceil_div(entries, static_cast<long long>(stream ? kRowsWaves / 2 : kRowsWaves));
+    if (!launchable(blocks, kRowsBlock)) return fail(1, "%s: too much work for one launch", who);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        auto go = [&](auto stream) {
-            expert_sum_backward_kernel<T, stream><<<dim3(static_cast<unsigned>(ceil_div(entries, static_cast<long long>(kRowsWaves)))), dim3(kRowsBlock), 0, s>>>(
+        auto go = [&](auto streaming) {
+            expert_sum_backward_kernel<T, streaming><<<dim3(static_cast<unsigned>(blocks)), dim3(kRowsBlock), 0, s>>>(
                 static_cast<const T*>(dout), ldd, static_cast<const T*>(y), ldy, weights, slots, static_cast<int>(n_slots), static_cast<T*>(dy), lddy, dw, entries, k,
                 static_cast<int>(width));
         };
-        if (streams(n_slots, width, size)) go(std::true_type{});
-        else go(std::false_type{});
+        stream ? go(std::true_type{}) : go(std::false_type{});
         return check_launch("expert_sum_backward_kernel");
     });
 }

@@ -439,6 +439,27 @@ def test_row_moves_and_router_beyond_32_bit_offsets(prism):
     assert torch.equal(grad, prism.route_topk_backward(up, logits, want.weights, want.experts, renormalise=False))
 
 
+@pytest.mark.parametrize("dtype,slots_of_all,width", [(torch.bfloat16, 13001, 8197), (torch.float32, 6700, 8192)])
+def test_rows_beyond_the_caches(prism, dtype, slots_of_all, width):
+    tokens, k = 301, 3
+    gen = torch.Generator(device=DEV).manual_seed(width)
+    slots = torch.randperm(slots_of_all, generator=gen, device=DEV)[:tokens * k].int().view(tokens, k).contiguous()
+    slots[5], slots[6, 1] = -1, -1
+    used = torch.zeros(slots_of_all, dtype=torch.bool, device=DEV)
+    used[slots[slots >= 0].long()] = True
+    y = normal(1, slots_of_all, width).to(dtype)
+    y[~used] = math.nan
+    up, w = normal(2, tokens, width).to(dtype), normal(3, tokens, k)
+    picked = torch.where((slots >= 0)[..., None], y[slots.clamp(min=0).long()].double(), 0.0)
+    near(prism.expert_combine(y, w, slots), (picked * w.double()[..., None]).sum(1), (picked * w.double()[..., None]).abs().sum(1), k + 2)
+    grad_y, grad_w = prism.expert_combine_backward(up, y, w, slots, grad_y=torch.full_like(y, -7.0))
+    dots = picked * up.double()[:, None]
+    near(grad_w, dots.sum(2), dots.abs().sum(2), width + 8)
+    want = w.double()[..., None] * up.double()[:, None]
+    near(grad_y[slots[slots >= 0].long()], want[slots >= 0], want[slots >= 0].abs(), 1)
+    assert bool((grad_y[~used] == -7).all())
+
+
 def test_no_tokens_or_no_slots(prism):
     none = lambda *s, dtype=torch.float32: torch.empty(s, dtype=dtype, device=DEV)  # noqa: E731
     r = prism.route_topk(none(0, 8), 2)
