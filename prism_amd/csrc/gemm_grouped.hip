@@ -12,6 +12,12 @@
 //
 // What a tile reads beyond its rows, columns or c arrives as zero: rows of other groups never enter a sum, whatever
 // they hold.
+//
+// 2 R N K flop. With many rows a group the matrix pipe bounds them, with few reading B (at 1.4 PFLOP/s and 6 TB/s both take as
+// long at some 230 rows). Three kernels (choose_kernel):
+// 16, 128 or 256 rows a tile. bf16, 2048 x 4096 matrices: forward 65536 rows of 64 groups 880 us (1.25 PFLOP/s; the dense
+// product of this library reaches 1.5), grad_a 32768 rows of 32 groups 478 us (1.15), grad_b of the same 606 us (0.91, and
+// 1.07 GB of fp32 results). 32 rows of 64 groups, 1536 x 2048, at most 160 MB of B: 30 us (5.3 TB/s).
 #include <type_traits>
 
 #include "common.h"
@@ -170,7 +176,9 @@ __device__ __forceinline__ void load_packets(uint16_t* tile, const OperandSource
 
 // ------------------------------------------------------------------------------------------- the general kernel --
 // 128 x 128 tiles, four waves of 64 x 64, one tile a workgroup: operands of any alignment, and problems with too few big
-// tiles for the chip. RAGGED_C: the groups lie along c (grad_b).
+// tiles for the chip. RAGGED_C: the groups lie along c (grad_b). Bound by what feeds the matrix pipe: a stage is 32 KiB into
+// LDS and 64 KiB out of it for 0.21 us of matrix instructions. 5003 rows of 24 groups by 1000 x 1048, fp32 results: 28.5 us
+// (0.37 PFLOP/s).
 // Direct-to-LDS loads into a ring of STAGES stages of 64 c. Four, three ahead, where there is a tile to a CU and nothing else
 // hides the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of 0.45); two where
 // there are more tiles and two workgroups share a CU (choose_kernel). Not ALIGNED: the last stage, or every one of rows too
@@ -290,6 +298,10 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
 //   * an accumulator is read by nothing but that instruction within 64 clocks of its last one (grouped_settle);
 //   * a fragment register written by the vector ALU is not used by the next few instructions (s_nop at the loop's head);
 //   * descriptors and scalar offsets are in scalar registers well before the load that reads them.
+// Bound by the matrix pipe: a stage takes 1.35 us (straight operands; 1.45 turned), a tile 9 to 12 us besides: its first
+// fragments, half-empty last row tiles of the groups, and the write-back, which a CU's next tile waits for where all CUs write
+// at once (in-order waits). Tried: non-temporal stores (+1 % on grad_b), other paces of the turned reads, staggered starts
+// (slower).
 // New here: every load goes through its descriptor's extent, which ends with the group (straight: the lines that exist;
 // turned: the c that exist), so that ragged tiles need no code of their own, and the walk over the tiles of all groups
 // reads a table that the workgroup makes of the offsets in LDS at its start.
@@ -719,7 +731,8 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
 // ------------------------------------------------------------------------------------------- few rows: 16 a tile --
 // The forward product where a group has few rows: reading B bounds it. A wavefront takes 16 columns and a slice of K, 128 k
 // to a step; its lane reads 16 B of the column's row of B for every instruction (the four lanes of a row 64 B, the next
-// instruction's the rest of the line), so the rows need no alignment. `parts` of a column tile meet in LDS.
+// instruction's the rest of the line), so the rows need no alignment. The parts of a column tile meet in LDS. 64 matrices of
+// 1536 x 2048, 32 rows: 30 us, 5.3 TB/s.
 constexpr int kFewWaves = 8, kFewLeast = 2, kFewStep = 128;
 
 struct FewProblem {

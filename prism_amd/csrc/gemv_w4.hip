@@ -13,6 +13,10 @@
 //   * that pattern is the bf16 number 16 + q, exactly: what it adds is taken off per group of G, as
 //     (16 + z) * (sum of x over the group), whose sums come from the same instruction on a matrix of ones;
 //   * the scale is applied to a group's fp32 sum, not to the weights. Nothing is rounded below 32 bits but the result.
+// Kernel times: 8192 x 8192, G = 128, 1 row: 9.8 us (34.6 MB, 3.5 TB/s); 16384 x 16384: 30.2 us (4.6 TB/s); 64 matrices of
+// 1536 x 2048, G = 32 with zero points, 32 rows: 17.7 us. What is left is latency: two rounds of loads in flight a wavefront, three to
+// six rounds a slice, and some 4 us in which the first weights arrive and the parts meet. x in LDS (+2 to 5 us), sixteen
+// wavefronts a workgroup, all of K up front and non-temporal loads (+1.4 us) were slower.
 #include <type_traits>
 
 #include "common.h"

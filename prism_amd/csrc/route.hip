@@ -9,6 +9,10 @@
 //   plan      entries (t, j) = t k + j in the order of their experts, equal experts in the order of the entries:
 //             offsets[e] entries go to experts below e, rows[s] is the entry in slot s, slots[t][j] its inverse.
 // Ranks come from counts and from positions inside a wavefront, never from the order in which atomics arrive.
+//
+// Launches and dependent steps bound it, not bytes. Router and plan: 1 token, 64 experts, k = 4: one kernel of 4.9 us (7.4 us
+// a call from Python); 16384 tokens, 256 experts bf16, k = 8: choice and counts 8.3 us (8.4 MB; eight rounds of a 16-lane
+// maximum), sums 4.7, places 5.8, together 17 us with their launches overlapping. Gradient of 32768 x 128 fp32: 8.3 us, 4.2 TB/s.
 #include <cmath>
 #include <type_traits>
 
@@ -264,12 +268,13 @@ __device__ __forceinline__ void scan_experts(int* value, int experts) {
     __syncthreads();
 }
 
-// One workgroup does the whole plan up to here: its counters fit 64 KiB of LDS.
 // One workgroup of 16 wavefronts does a run of up to kRun entries: counts them per wavefront in LDS, sums the counts over
 // the wavefronts, places them. A plan of one run takes the experts' offsets from its own counts; in longer ones they come
 // from the counts of all runs (plan_count_kernel), which every run adds up for itself, or, with many runs, plan_sum_kernel.
 constexpr int kRunWaves = 16, kRun = 4096, kShortRun = 512;
-constexpr int kSelfSum = 32;  // runs up to which each adds up all counts
+// Runs up to which each adds up all counts. Router and plan, 64 experts, k = 4, this way / with plan_sum_kernel: 33 runs 9.2 / 10.8 us,
+// 63 runs 11.7 / 11.1.
+constexpr int kSelfSum = 48;
 
 __device__ __forceinline__ void count_run(const int32_t* chosen, int first, int end, int per, int experts, int* count) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(kRunWaves * kWave) void plan_small_kernel(const int
     plan_in_workgroup(chosen, entries, experts, bits, offsets, rows, slots, plan_lds);
 }
 
-// Router and plan of up to 64 tokens (16 lanes each) in one launch.
+// Router and plan of up to 64 tokens (16 lanes each) in one launch (1 token: 4.8 us a call from C, 7.0 as two).
 template <typename T, int VALUES, int PACK>
 __global__ __launch_bounds__(kRunWaves * kWave) void route_small_kernel(const T* logits, long long ld, int tokens, int experts, int k, int renormalise,
                                                                         float* weights, int32_t* chosen, int bits, int32_t* offsets, int32_t* rows,
@@ -351,7 +356,8 @@ __global__ __launch_bounds__(kRunWaves * kWave) void plan_count_kernel(const int
     for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[static_cast<long long>(blockIdx.x) * experts + e] = plan_lds[e];
 }
 
-// Router of 64 tokens a workgroup, and their counts: the plan's first step rides along.
+// Router of 64 tokens a workgroup, and their counts: the plan's first step rides along (16384 tokens, 256 experts,
+// k = 8: 17.2 us with its plan, 19.0 as calls of their own).
 template <typename T, int VALUES, int PACK>
 __global__ __launch_bounds__(kRunWaves * kWave) void route_count_kernel(const T* __restrict__ logits, long long ld, int tokens, int experts, int k, int renormalise,
                                                                         float* weights, int32_t* chosen, int* __restrict__ counts) {
@@ -408,6 +414,7 @@ __global__ __launch_bounds__(kRunWaves * kWave) void plan_place_kernel(const int
             before = counts[static_cast<long long>(blockIdx.x) * experts + e];
             total = totals[e];
         } else {
+#pragma unroll 8  // loads under way at a time: 2000 tokens, 64 experts, k = 4, 32 runs: 15.9 -> 9.0 us
             for (int r = 0; r < runs; ++r) {
                 const int c = counts[static_cast<long long>(r) * experts + e];
                 before += r < static_cast<int>(blockIdx.x) ? c : 0;
