@@ -385,17 +385,18 @@ int prism_runmyh100(int M, int N, int K, const uint16_t* A, const uint16_t* B,
  *
  * Shared rules. Element types are PRISM_TYPE_*; bf16 values are 16-bit
  * patterns. ld* are the elements between rows of a row-major matrix, at least
- * a row's length; pointers need the alignment of their elements only (bases and
- * rows that are multiples of 16 bytes are faster). Outputs must not overlap
- * inputs, from a matrix' first element to its last. Sizes stay below 2^31 - 4096 and
- * a call's launch below 2^32 threads (a row move: 64 GiB of rows); what does
- * not is refused. offsets is a group table in device memory, groups + 1 entries: group
- * g owns the rows offsets[g] .. offsets[g + 1] - 1 of the row operand (empty
- * groups are fine); rows outside [offsets[0], offsets[groups]) are neither used
- * nor written. Table, slot and row entries are cut to the buffers given, so
- * wrong ones give wrong results but no access outside. Sums run in 32 bits, in
- * an order that does not change from run to run. The calls allocate nothing,
- * keep nothing and may be captured into HIP graphs.
+ * a row's length; pointers need the alignment of their elements only (bases
+ * and rows that are multiples of 16 bytes are faster). Outputs must not
+ * overlap inputs, from a matrix' first element to its last. Sizes stay below
+ * 2^31 - 4096 and a call's launch below 2^32 threads (a row move: 64 GiB of
+ * rows); what does not is refused. offsets is a group table in device memory,
+ * groups + 1 entries: group g owns the rows offsets[g] .. offsets[g + 1] - 1
+ * of the row operand (empty groups are fine); rows outside [offsets[0],
+ * offsets[groups]) are neither used nor written. Table, slot and row entries
+ * are cut to the buffers given, so wrong ones give wrong results but no access
+ * outside. Sums run in 32 bits, in an order that does not change from run to
+ * run. The calls allocate nothing, keep nothing and may be captured into HIP
+ * graphs.
  */
 enum { PRISM_TYPE_F32 = 0, PRISM_TYPE_BF16 = 1 };
 
@@ -498,14 +499,15 @@ int prism_gemm_bf16_grouped_grad_b(int groups, int64_t rows, int N, int K, const
                                    void* dB, int64_t ldb, int64_t group_stride, int b_type, void* stream);
 
 /*
- * A few rows times weights held in 4 bits: y[r][n] = sum_k x[r][k]
- * scales[n][k / group_size] (q[n][k] - zeros[n][k / group_size]) for the rows of
- * group g and its matrix. x: rows x K bf16, finite (an infinity gives NaN: the
- * kernel works with 16 + q and takes 16 + zeros off again). q: groups matrices of N rows of (K + 1) / 2 bytes, two weights to a byte, the even k in the low nibble; ldq
- * and group_stride in bytes. scales (bf16) and zeros (uint8, NULL: 8
- * throughout): groups x N x ceil(K / group_size), contiguous; group_size a
- * multiple of 32. offsets may be NULL for one matrix: all rows use it. y: rows x
- * N of y_type. Made for up to 16 rows a group; more are right, and fetch the
+ * A few rows times weights held in 4 bits: y[r][n] = sum_k x[r][k] scales[n][k
+ * / group_size] (q[n][k] - zeros[n][k / group_size]) for the rows of group g
+ * and its matrix. x: rows x K bf16, finite (an infinity gives NaN: the kernel
+ * works with 16 + q and takes 16 + zeros off again). q: groups matrices of N
+ * rows of (K + 1) / 2 bytes, two weights to a byte, the even k in the low
+ * nibble; ldq and group_stride in bytes. scales (bf16) and zeros (uint8, NULL:
+ * 8 throughout): groups x N x ceil(K / group_size), contiguous; group_size a
+ * multiple of 32. offsets may be NULL for one matrix: all rows use it. y: rows
+ * x N of y_type. Made for up to 16 rows a group; more are right, and fetch the
  * weights once per 16 rows (from the L2 after the first).
  */
 int prism_gemv_w4(int groups, int64_t rows, int N, int K, const uint16_t* x, int64_t ldx,

@@ -874,7 +874,7 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
     p.groups = g.groups; p.rows = g.rows; p.N = g.cols; p.K = g.depth;
     const long long row_tiles = most_row_tiles(g.rows, g.groups, 16);
     p.row_tiles = static_cast<int>(row_tiles);
-    p.k_parts = few_rows_k_parts(g.rows < g.groups ? g.rows : row_tiles, p.N, p.K, kFewStep, kFewWaves, 16);
+    p.k_parts = few_rows_k_parts(busy_row_tiles(g.rows, g.groups, row_tiles), p.N, p.K, kFewStep, kFewWaves, 16);
     p.n_parts = p.k_parts < kFewLeast ? kFewLeast / p.k_parts : 1;
     p.tiles_n = ceil_div(p.N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;

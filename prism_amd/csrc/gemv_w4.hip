@@ -14,7 +14,7 @@
 //     (16 + z) * (sum of x over the group), whose sums come from the same instruction on a matrix of ones;
 //   * the scale is applied to a group's fp32 sum, not to the weights. Nothing is rounded below 32 bits but the result.
 // Kernel times: 8192 x 8192, G = 128, 1 row: 9.8 us (34.6 MB, 3.5 TB/s); 16384 x 16384: 30.2 us (4.6 TB/s); 64 matrices of
-// 1536 x 2048, G = 32 with zero points, 32 rows: 17.7 us. What is left is latency: two rounds of loads in flight a wavefront, three to
+// 1536 x 2048, G = 32 with zero points, 32 rows: 17 us. What is left is latency: two rounds of loads in flight a wavefront, three to
 // six rounds a slice, and some 4 us in which the first weights arrive and the parts meet. x in LDS (+2 to 5 us), sixteen
 // wavefronts a workgroup, all of K up front and non-temporal loads (+1.4 us) were slower.
 #include <type_traits>
@@ -42,6 +42,7 @@ struct W4Problem {
     int groups, rows, N, K, G, n_groups;          // n_groups: scales per row
     int tiles_n, row_tiles;  // workgroups along N, tiles of 16 rows
     int k_parts, n_parts; // wavefronts that share a column tile's K, column tiles of a workgroup
+    int slice;            // steps of such a wavefront
 };
 
 __device__ __forceinline__ void store_y(float* p, float v) { *p = v; }
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Problem p) 
     s.rows = row_end - row0 < 16 ? row_end - row0 : 16;
     s.whole = p.K / kW4Block;
     s.steps = (p.K + kW4Block - 1) / kW4Block;
-    s.slice = (s.steps + p.k_parts - 1) / p.k_parts;
+    s.slice = p.slice;
     s.first = k_part * s.slice;
     s.K = p.K;
     s.G = p.G;
@@ -345,13 +346,14 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
         meets(offsets, (static_cast<uintptr_t>(groups) + 1) * 4))
         return fail(1, "%s: the output overlaps an input", who);
     const long long row_tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16) : ceil_div(rows, 16ll);
-    // Of a group table's tiles about as many exist as there are rows or groups.
-    const long long busy = offsets != nullptr ? (rows < groups ? rows : row_tiles) : row_tiles;
+    const long long busy = offsets != nullptr ? busy_row_tiles(rows, groups, row_tiles) : row_tiles;
     // Twelve wavefronts a CU, none with less than a round of few rows (512 k: shorter slices only have the loop's last,
     // unpipelined part). Against eight and single steps: 16384 x 16384 by 1 row 35.6 -> 30.2 us, 8192 x 1024 by 16 rows 7.1 -> 5.3,
-    // 2048 x 1024 by 4 rows 5.0 -> 3.7, none of sixteen sizes slower by 1 %; sixteen wavefronts gain 7 % on 64 matrices of
-    // 1536 x 2048 by 32 rows but lose 40 % on 14336 x 4096 by 1 row (9.1 -> 13.0 us) and 19 % on 8 of 2048 x 2048 by 64.
+    // 2048 x 1024 by 4 rows 5.0 -> 3.7, none of sixteen sizes slower by 1 %; sixteen wavefronts lose 40 % on
+    // 14336 x 4096 by 1 row (9.1 -> 13.0 us) and 19 % on 8 matrices of 2048 x 2048 by 64 rows.
     p.k_parts = few_rows_k_parts(busy, N, K, 4 * kW4Block, kW4Waves, 12);
+    // Whole rounds: only the last slice has steps outside the pipeline (5120 x 5120 by 4 rows, groups of 128: 13.3 -> 8.4 us).
+    p.slice = ceil_div(ceil_div(ceil_div(K, kW4Block), p.k_parts), 4) * 4;
     p.n_parts = p.k_parts < kW4Few ? kW4Few / p.k_parts : 1;
     p.tiles_n = ceil_div(N, 16 * p.n_parts);
     const long long blocks = row_tiles * ceil_div(p.tiles_n, kXcds) * kXcds;

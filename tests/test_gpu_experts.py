@@ -546,6 +546,30 @@ def test_a_layer_captured_and_replayed(prism):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("tokens,experts,k", [(1100, 64, 4), (2900, 64, 4), (5000, 40, 5), (9001, 1024, 3), (4100, 520, 1)])
+def test_routes_of_many_tokens_captured(prism, tokens, experts, k):
+    """Two graphs, each with its own results and workspaces, replayed in turn with other calls between; every replay against the eager call."""
+    logits = [normal(i, tokens, experts).bfloat16() for i in range(4)]
+    inputs = [x.clone() for x in logits[:2]]
+    for z in logits:
+        r = prism.route_topk(z, k)
+        want = torch.topk(z.float(), k).values
+        assert torch.equal(z.float().gather(1, r.experts.long()), want)
+        assert all(torch.equal(a, b) for a, b in zip(r[2:], plain_plan(r.experts, experts)))
+    graphs, got = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g, z in zip(graphs, inputs):
+        with torch.cuda.graph(g):
+            got.append(prism.route_topk(z, k))
+    for turn in range(3):
+        for i in (0, 1):
+            inputs[i].copy_(logits[(turn + i) % 4])
+            graphs[i].replay()
+        between = prism.route_topk(logits[3], k)
+        for i in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(got[i], prism.route_topk(logits[(turn + i) % 4], k)))
+        assert all(torch.equal(a, b) for a, b in zip(between, prism.route_topk(logits[3], k)))
+
+
 def test_large_plans_in_graphs_and_on_two_streams(prism):
     """The plan with a workspace: captured, and two at once on two streams."""
     choices = [torch.randint(0, 64, (9000, 4), device=DEV, dtype=torch.int32) for _ in range(2)]
