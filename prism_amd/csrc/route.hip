@@ -12,7 +12,7 @@
 //
 // Launches and dependent steps bound it, not bytes. Router and plan: 1 token, 64 experts, k = 4: one kernel of 4.9 us (7.4 us
 // a call from Python); 16384 tokens, 256 experts bf16, k = 8: choice and counts 8.3 us (8.4 MB; eight rounds of a 16-lane
-// maximum), sums 4.7, places 5.8, together 17 us with their launches overlapping. Gradient of 32768 x 128 fp32: 8.3 us, 4.2 TB/s.
+// maximum), sums 4.7, places 5.8, together 17 us with their launches overlapping. Gradient of 32768 x 128 fp32: 8.3 us, 4.4 TB/s.
 #include <cmath>
 #include <type_traits>
 
