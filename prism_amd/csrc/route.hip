@@ -72,7 +72,7 @@ __device__ __forceinline__ float logit_of(uint32_t o) { return __builtin_bit_cas
 constexpr uint32_t kOrderNone = 0x007fffffu;  // order_of(-inf): this and below is not there
 
 // One token by the 16 lanes of a row, VALUES logits each: value v of a lane is expert (v / PACK) 16 PACK + lane PACK + v % PACK.
-// Picking is k rounds of: the row's largest key, its expert, its key struck out. bf16: the key holds the order in its upper
+// Picking is k rounds of: the row's largest key that is left, its expert. bf16: the key holds the order in its upper
 // half and the complement of the expert in its lower one, so that one maximum finds both; fp32: the order is the key, the
 // lowest expert that has it is found by a second maximum (of complements).
 template <typename T, int VALUES, int PACK>
@@ -99,18 +99,19 @@ __device__ __forceinline__ void choose_experts(const T* z, int experts, int k, b
     // Lane j keeps the j-th and the (j + 16)-th.
     uint32_t my_key[2] = {0u, 0u};
     int my_expert[2] = {-1, -1};
-    uint32_t top = 0;
+    uint32_t top = 0, last = 0;
     for (int j = 0; j < k; ++j) {
-        uint32_t best = key[0];
+        // PACKED: the largest key below the last one. Relative to that one and modulo 2^32, the keys from it on are small and
+        // those below it large, in their order: a subtraction each, and nothing is struck out.
+        uint32_t best = key[0] - last;
 #pragma unroll
-        for (int v = 1; v < VALUES; ++v) best = max(best, key[v]);
-        const uint32_t won = row_max(best);
+        for (int v = 1; v < VALUES; ++v) best = max(best, key[v] - last);
+        const uint32_t won = row_max(best) + last;
         if (won == 0) break;  // the same for the 16 lanes
         int expert;
         if constexpr (PACKED) {
             expert = static_cast<uint16_t>(~won);
-#pragma unroll
-            for (int v = 0; v < VALUES; ++v) key[v] = key[v] == won ? 0u : key[v];  // keys differ: it is this expert's
+            last = won;
         } else {
             uint32_t other = 0;  // complement of the lowest expert with this order, among this lane's
 #pragma unroll
@@ -135,7 +136,7 @@ __device__ __forceinline__ void choose_experts(const T* z, int experts, int k, b
     }
     if (!renormalise)  // and those that were not chosen
 #pragma unroll
-        for (int v = 0; v < VALUES; ++v) total += key[v] ? expf(logit(key[v]) - z0) : 0.0f;
+        for (int v = 0; v < VALUES; ++v) total += key[v] != 0u && (!PACKED || key[v] < last) ? expf(logit(key[v]) - z0) : 0.0f;
     total = row_sum(total);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -292,11 +293,13 @@ __device__ __forceinline__ void place_run(const int32_t* chosen, int first, int 
                                           int total, int32_t* rows, int32_t* slots) {
     const int wave = threadIdx.x / kWave;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-        int next = start[e];
+        int next = start[e], c[kRunWaves];  // all read before the first is written: one LDS latency, not sixteen
+#pragma unroll
+        for (int w = 0; w < kRunWaves; ++w) c[w] = count[w * experts + e];
+#pragma unroll
         for (int w = 0; w < kRunWaves; ++w) {
-            const int c = count[w * experts + e];
             count[w * experts + e] = next;
-            next += c;
+            next += c[w];
         }
     }
     __syncthreads();
@@ -377,26 +380,44 @@ __global__ __launch_bounds__(kRunWaves * kWave) void route_count_kernel(const T*
 }
 
 // counts[run][expert] becomes its sum over the runs before; totals[expert] the sum over all. 16 experts a workgroup, the
-// runs in 64 parts.
+// runs in 64 parts, four to a wavefront. A part's first counts stay in registers, loaded all at a time.
 __global__ __launch_bounds__(1024) void plan_sum_kernel(int* __restrict__ counts, int runs, int experts, int* __restrict__ totals) {
-    __shared__ int part_sum[64][17];
-    const int e = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16;
-    const int per = (runs + 63) / 64, first = min(part * per, runs), end = min(first + per, runs);
-    int sum = 0;
-    if (e < experts)
-        for (int c = first; c < end; ++c) sum += counts[static_cast<long long>(c) * experts + e];
-    part_sum[part][threadIdx.x % 16] = sum;
+    constexpr int WAVES = 16, HELD = 8;
+    __shared__ int wave_sum[WAVES][16];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, l16 = lane % 16;
+    const int e = blockIdx.x * 16 + l16, part = threadIdx.x / 16;
+    const int per = (runs + 63) / 64, first = min(part * per, runs), end = e < experts ? min(first + per, runs) : first;
+    int* at = counts + static_cast<long long>(first) * experts + e;  // of run `first`
+    int held[HELD], sum = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        held[i] = first + i < end ? at[static_cast<long long>(i) * experts] : 0;
+        sum += held[i];
+    }
+#pragma unroll 8
+    for (int i = HELD; i < end - first; ++i) sum += at[static_cast<long long>(i) * experts];
+    int upto = sum;
+#pragma unroll
+    for (int d = 16; d < kWave; d *= 2) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane >= kWave - 16) wave_sum[wave][l16] = upto;
     __syncthreads();
-    if (e >= experts) return;
-    int before = 0;
-    for (int r = 0; r < part; ++r) before += part_sum[r][threadIdx.x % 16];
-    for (int c = first; c < end; ++c) {
-        const long long at = static_cast<long long>(c) * experts + e;
-        const int v = counts[at];
-        counts[at] = before;
+    int before = upto - sum;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) before += w < wave ? wave_sum[w][l16] : 0;
+    if (e < experts && part == 63) totals[e] = before + sum;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        if (first + i < end) at[static_cast<long long>(i) * experts] = before;
+        before += held[i];
+    }
+    for (int i = HELD; i < end - first; ++i) {
+        const int v = at[static_cast<long long>(i) * experts];
+        at[static_cast<long long>(i) * experts] = before;
         before += v;
     }
-    if (part == 63) totals[e] = before;
 }
 
 // totals == nullptr: counts are the runs' own, and this run adds them up.
