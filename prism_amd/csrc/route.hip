@@ -10,9 +10,9 @@
 //             offsets[e] entries go to experts below e, rows[s] is the entry in slot s, slots[t][j] its inverse.
 // Ranks come from counts and from positions inside a wavefront, never from the order in which atomics arrive.
 //
-// Launches and dependent steps bound it, not bytes. Router and plan: 1 token, 64 experts, k = 4: one kernel of 4.9 us (7.4 us
-// a call from Python); 16384 tokens, 256 experts bf16, k = 8: choice and counts 8.3 us (8.4 MB; eight rounds of a 16-lane
-// maximum), sums 4.7, places 5.8, together 17 us with their launches overlapping. Gradient of 32768 x 128 fp32: 8.3 us, 4.4 TB/s.
+// Launches and dependent steps bound it, not bytes. Router and plan: 1 token, 64 experts, k = 4: one kernel of 4.5 us (7.7 us
+// a call from Python); 16384 tokens, 256 experts bf16, k = 8: choice and counts 7.4 us (8.4 MB; eight rounds of a 16-lane
+// maximum), sums 3.3, places 5.8, together 14.7 us (bf16 keys struck out one by one and counts summed one by one: 17.2). Gradient of 32768 x 128 fp32: 8.3 us, 4.4 TB/s.
 #include <cmath>
 #include <type_traits>
 
@@ -273,8 +273,8 @@ __device__ __forceinline__ void scan_experts(int* value, int experts) {
 // the wavefronts, places them. A plan of one run takes the experts' offsets from its own counts; in longer ones they come
 // from the counts of all runs (plan_count_kernel), which every run adds up for itself, or, with many runs, plan_sum_kernel.
 constexpr int kRunWaves = 16, kRun = 4096, kShortRun = 512;
-// Runs up to which each adds up all counts. Router and plan, 64 experts, k = 4, this way / with plan_sum_kernel: 33 runs 9.2 / 10.8 us,
-// 63 runs 11.7 / 11.1.
+// Runs up to which each adds up all counts. Router and plan, 64 experts, k = 4, this way / with plan_sum_kernel: 32 runs 8.6 /
+// 10.2 us, 40 runs 8.9 / 10.2, 63 runs 11.0 / 10.2.
 constexpr int kSelfSum = 48;
 
 __device__ __forceinline__ void count_run(const int32_t* chosen, int first, int end, int per, int experts, int* count) {
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(kRunWaves * kWave) void plan_count_kernel(const int
 }
 
 // Router of 64 tokens a workgroup, and their counts: the plan's first step rides along (16384 tokens, 256 experts,
-// k = 8: 17.2 us with its plan, 19.0 as calls of their own).
+// k = 8: 14.7 us with its plan, 16.5 as calls of their own).
 template <typename T, int VALUES, int PACK>
 __global__ __launch_bounds__(kRunWaves * kWave) void route_count_kernel(const T* __restrict__ logits, long long ld, int tokens, int experts, int k, int renormalise,
                                                                         float* weights, int32_t* chosen, int* __restrict__ counts) {
