@@ -890,20 +890,23 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
 //   general  rounds of 256 tiles of 128 x 128 at 4 + 0.48 a stage with a ring of four stages, of 512 at 4 + 1.1 with one of
 //            two, or B once at 4.3 TB/s
 //   big      rounds of 256 tiles of 256 x 256 at 8 + 1.2 a stage (stages in pairs), or B once at 4.3 TB/s
+// (gradient of B: instead of B, results beyond the memory-side cache at 5.3 TB/s from big tiles and 4.2 from general ones).
 // Measured, few / general / big: 64 rows of 32 groups, 2048 x 2048: 56 / 57 / 65 us; 512 rows: 101 / 63 / 70; 2048 rows:
 // 252 / 67 / 73; 8192 rows: - / 106 / 82; 100 rows of 8 groups, 256 x 4096: 10 / 34 / 69; 2000 rows of 16, 768 x 768: 38 /
 // 12 / 21. Gradient of B, general / big: 512 rows of 32 groups, 2048 x 2048: 137 / 66; 1000 rows of 32, 304 x 512: 10 / 12.
 // General, four stages / two: 5003 rows of 24 groups, 1000 x 1048: 32.9 / 28.7; 4000 of 8, 2048 x 1024: 30.4 / 25.3; 2000 of 16,
-// 768 x 768: 12.2 / 13.4; 6000 of 16, 1536 x 2048: 79 / 83; gradient of B, 1000 rows of 32, 304 x 512: 10.0 / 7.8.
+// 768 x 768: 12.2 / 13.4; 6000 of 16, 1536 x 2048: 79 / 83; gradient of B, 1000 rows of 32, 304 x 512: 10.0 / 7.8. Gradient
+// of B, two / big: 1000 rows of 64, 2048 x 1024, 537 MB: 127 / 102; 717 of 64, 704 x 1216: 46 / 51.
 enum class Kernel { kFew, kGeneral, kGeneralPairs, kBig };
 template <bool RAGGED_C>
-Kernel choose_kernel(const GroupedProblem& g, bool can_few, bool can_big) {
+Kernel choose_kernel(const GroupedProblem& g, int out_size, bool can_few, bool can_big) {
     const double rows = g.rows, groups = g.groups, used = rows < groups ? rows : groups;
     auto row_tiles = [&](double tile) { const double t = rows / tile + used / 2; return t > used ? t : used; };
     auto rounds = [](double tiles) { return static_cast<double>(static_cast<long long>((tiles + 255.0) / 256.0)); };
     const double depth = RAGGED_C ? rows / groups : static_cast<double>(g.depth), stages = static_cast<double>(static_cast<long long>((depth + 63) / 64));
-    const double b_us = RAGGED_C ? 0.0 : used * g.cols * depth * 2 / 4.3e6;
+    const double results = RAGGED_C ? groups * g.out_rows * g.cols * out_size : 0.0;
     auto tiled = [&](int edge, int per_cu, double fixed, double stage_us, double n_stages) {
+        const double b_us = !RAGGED_C ? used * g.cols * depth * 2 / 4.3e6 : (results > (256 << 20) ? results / (edge == 256 ? 5.3e6 : 4.2e6) : 0.0);
         const double tiles = (RAGGED_C ? groups * ceil_div(g.out_rows, edge) : row_tiles(edge)) * ceil_div(g.cols, edge);
         const double us = rounds(tiles / per_cu) * (fixed + stage_us * n_stages);
         return 2 + (us > b_us ? us : b_us);
@@ -926,7 +929,7 @@ int run(GroupedProblem g, const char* who, hipStream_t s) {
     const int p_along = P_TURNED ? g.out_rows : g.depth, q_along = Q_TURNED ? g.cols : g.depth;
     const bool aligned = aligned16(g.P) && aligned16(g.Q) && g.ldp % 8 == 0 && g.ldq % 8 == 0 && (RAGGED_C || g.group_stride % 8 == 0) &&
                          p_along % 8 == 0 && q_along % 8 == 0 && g.near;
-    const Kernel kernel = choose_kernel<RAGGED_C>(g, FORWARD, aligned && g.groups <= kBigGroups && cu_count() >= 8);
+    const Kernel kernel = choose_kernel<RAGGED_C>(g, static_cast<int>(sizeof(OutT)), FORWARD, aligned && g.groups <= kBigGroups && cu_count() >= 8);
     if constexpr (FORWARD)
         if (kernel == Kernel::kFew) return run_few<OutT>(g, who, s);
     const int edge = kernel == Kernel::kBig ? 256 : 128;
