@@ -501,10 +501,10 @@ int prism_gemm_bf16_grouped_grad_b(int groups, int64_t rows, int N, int K, const
 /*
  * A few rows times weights held in 4 bits: y[r][n] = sum_k x[r][k] scales[n][k
  * / group_size] (q[n][k] - zeros[n][k / group_size]) for the rows of group g
- * and its matrix. x: rows x K bf16, finite (an infinity gives NaN: the kernel
- * works with 16 + q and takes 16 + zeros off again). q: groups matrices of N
- * rows of (K + 1) / 2 bytes, two weights to a byte, the even k in the low
- * nibble; ldq and group_stride in bytes. scales (bf16) and zeros (uint8, NULL:
+ * and its matrix. x: rows x K bf16, any finite numbers (an infinity gives
+ * NaN: the kernel works with 16 + q and takes 16 + zeros off again). q: groups
+ * matrices of N rows of (K + 1) / 2 bytes, two weights to a byte, the even k in
+ * the low nibble; ldq and group_stride in bytes. scales (bf16) and zeros (uint8, NULL:
  * 8 throughout): groups x N x ceil(K / group_size), contiguous; group_size a
  * multiple of 32. offsets may be NULL for one matrix: all rows use it. y: rows
  * x N of y_type. Made for up to 16 rows a group; more are right, and fetch the

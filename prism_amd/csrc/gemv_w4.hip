@@ -9,9 +9,11 @@
 //   * the order of k inside an instruction is free as long as both operands have the same: a lane takes 16 consecutive
 //     bytes of its row (32 weights; where groups are shorter than the 128 of a row's four lanes, the lanes exchange dwords
 //     so that an instruction stays inside a group), and the values of a dword in the order 0 4 1 5 2 6 3 7, in which
-//     `(w >> c) & 0x00780078 | 0x41804180` yields two of them;
-//   * that pattern is the bf16 number 16 + q, exactly: what it adds is taken off per group of G, as
-//     (16 + z) * (sum of x over the group), whose sums come from the same instruction on a matrix of ones;
+//     `(w >> c) & 0x00780078 | 0x39803980` yields two of them;
+//   * that pattern is the bf16 number 2^-16 (16 + q), exactly: what it adds is taken off per group of G, as
+//     (16 + z) * (sum of 2^-16 x over the group), whose sums come from the same instruction on a matrix of 2^-16. With that
+//     factor, taken back off the result, neither part overflows for any finite x (128 * 271 < 2^16) though x (q - z) does not,
+//     and products keep all their bits down to the smallest x (2^-133 2^-16 is fp32's smallest number);
 //   * the scale is applied to a group's fp32 sum, not to the weights. Nothing is rounded below 32 bits but the result.
 // Kernel times: 8192 x 8192, G = 128, 1 row: 9.8 us (34.6 MB, 3.5 TB/s); 16384 x 16384: 30.2 us (4.6 TB/s); 64 matrices of
 // 1536 x 2048, G = 32 with zero points, 32 rows: 17 us. What is left is latency: two rounds of loads in flight a wavefront, three to
@@ -48,9 +50,12 @@ struct W4Problem {
 __device__ __forceinline__ void store_y(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_y(uint16_t* p, float v) { *p = __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }
 
-// Eight weights of a dword as bf16 16 + q, in the order 0 4 1 5 2 6 3 7.
+// The results' factor of 2^-16 is taken off at the end.
+constexpr float kUnit = 65536.0f;
+
+// Eight weights of a dword as bf16 2^-16 (16 + q), in the order 0 4 1 5 2 6 3 7.
 __device__ __forceinline__ bf16x8 weights_of(uint32_t w) {
-    constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
+    constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x39803980u;
     u32x4 r;
     r[0] = ((w << 3) & kMask) | kSixteen;
     r[1] = ((w >> 1) & kMask) | kSixteen;
@@ -148,7 +153,7 @@ __device__ __forceinline__ f32x4 multiply_slice(const W4Slice& p) {
         }
     };
     f32x4 total = {0.0f, 0.0f, 0.0f, 0.0f};
-    const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    const u32x4 one = {0x37803780u, 0x37803780u, 0x37803780u, 0x37803780u};  // 2^-16
     const bf16x8 ones = __builtin_bit_cast(bf16x8, one);
     auto multiply = [&](u32x4 w, const bf16x8 (&x)[4], const uint16_t* s, const uint8_t* z) {
         if constexpr (TURN) w = turned(w);
@@ -297,7 +302,7 @@ __global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Problem p) 
     OutT* y = static_cast<OutT*>(p.y);
 #pragma unroll
     for (int v = 0; v < 4; ++v)
-        if (4 * lq + v < s.rows) store_y(y + (row0 + 4 * lq + v) * p.ldy + n0 + l16, total[v]);
+        if (4 * lq + v < s.rows) store_y(y + (row0 + 4 * lq + v) * p.ldy + n0 + l16, kUnit * total[v]);
 }
 
 template <StepScales SCALES>
