@@ -220,11 +220,12 @@ __global__ __launch_bounds__(256) void gemm_grouped_kernel(GroupedProblem g) {
     const int tiles = __builtin_amdgcn_readfirstlane(ps.depth > 0 ? (ps.depth + kBK - 1) / kBK : 1);  // without depth: a stage of zeros
     auto load = [&](int t) {  // beyond the last: zeros, so that every stage has its loads in flight
         uint16_t *to_p = Ps[t % STAGES], *to_q = Qs[t % STAGES];
-        // By ordinary loads, the stages before have landed as well when this one has (loads are waited for in order), and the
-        // counting in front of the barriers, which takes every stage's direct loads to be under way, errs to the safe side.
+        // The counting in front of the barriers takes every stage's direct loads to be under way. Where this one comes by ordinary
+        // loads, of which a wavefront may have none, the direct loads of the stages before are waited for here.
         if (!ALIGNED && t < tiles && (t == tiles - 1 || !g.near)) {
             load_packets<BM, P_TURNED, WAVES>(to_p, ps, t * kBK, wave, lane);
             load_packets<BN, Q_TURNED, WAVES>(to_q, qs, t * kBK, wave, lane);
+            __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kLgkmMax));
         } else {
             load_direct<BM, P_TURNED, WAVES>(to_p, ps, t * kBK, wave, lane);
             load_direct<BN, Q_TURNED, WAVES>(to_q, qs, t * kBK, wave, lane);
