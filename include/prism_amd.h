@@ -386,17 +386,17 @@ int prism_runmyh100(int M, int N, int K, const uint16_t* A, const uint16_t* B,
  * Shared rules. Element types are PRISM_TYPE_*; bf16 values are 16-bit
  * patterns. ld* are the elements between rows of a row-major matrix, at least
  * a row's length; pointers need the alignment of their elements only (bases
- * and rows that are multiples of 16 bytes are faster). Outputs must not
- * overlap inputs, from a matrix' first element to its last. Sizes stay below
- * 2^31 - 4096 and a call's launch below 2^32 threads (a row move: 64 GiB of
- * rows); what does not is refused. offsets is a group table in device memory,
- * groups + 1 entries: group g owns the rows offsets[g] .. offsets[g + 1] - 1
- * of the row operand (empty groups are fine); rows outside [offsets[0],
- * offsets[groups]) are neither used nor written. Table, slot and row entries
- * are cut to the buffers given, so wrong ones give wrong results but no access
- * outside. Sums run in 32 bits, in an order that does not change from run to
- * run. The calls allocate nothing, keep nothing and may be captured into HIP
- * graphs.
+ * and rows that are multiples of 16 bytes are faster). Outputs and workspaces
+ * that overlap inputs or each other, from a matrix' first element to its last,
+ * are refused. Sizes stay below 2^31 - 4096 and a call's launch below 2^32
+ * threads (a row move: 64 GiB of rows); what does not is refused. offsets is a
+ * group table in device memory, groups + 1 entries: group g owns the rows
+ * offsets[g] .. offsets[g + 1] - 1 of the row operand (empty groups are fine);
+ * rows outside [offsets[0], offsets[groups]) are neither used nor written.
+ * Table, slot and row entries are cut to the buffers given, so wrong ones give
+ * wrong results but no access outside. Sums run in 32 bits, in an order that
+ * does not change from run to run. The calls allocate nothing, keep nothing and
+ * may be captured into HIP graphs.
  */
 enum { PRISM_TYPE_F32 = 0, PRISM_TYPE_BF16 = 1 };
 

@@ -7,6 +7,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 
 namespace prism {
 
@@ -44,6 +45,31 @@ inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1
 
 template <typename T>
 constexpr T ceil_div(T a, T b) { return (a + b - 1) / b; }
+
+// Memory that a call reads or writes, and whether any of its outputs shares some with an input or another output.
+struct Span {
+    const void* at;
+    uintptr_t bytes;
+};
+// A row-major matrix, from its first element to its last.
+inline Span matrix_span(const void* at, long long rows, long long cols, long long ld, int size) {
+    return {at, rows <= 0 || cols <= 0 ? 0 : static_cast<uintptr_t>((rows - 1) * ld + cols) * size};
+}
+// An array of 4-byte entries.
+inline Span entries_span(const void* at, long long entries) { return {at, static_cast<uintptr_t>(entries) * 4}; }
+inline bool overlap(const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.at != nullptr && b.at != nullptr && a.bytes != 0 && b.bytes != 0 && x < y + b.bytes && y < x + a.bytes;
+}
+inline bool outputs_overlap(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+    for (const Span* o = outputs.begin(); o != outputs.end(); ++o) {
+        for (const Span& i : inputs)
+            if (overlap(*o, i)) return true;
+        for (const Span* p = outputs.begin(); p != o; ++p)
+            if (overlap(*o, *p)) return true;
+    }
+    return false;
+}
 
 // Compute units of the current device (the launchers size their tile choices by it).
 inline int cu_count() {

@@ -175,11 +175,6 @@ int check_rows(const char* who, int type, long long tokens, int k, long long n_s
     }
     return 0;
 }
-bool rows_overlap(const void* a, long long a_rows, long long lda, const void* b, long long b_rows, long long ldb, long long width, int size) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    const uintptr_t xs = static_cast<uintptr_t>((a_rows - 1) * lda + width) * size, ys = static_cast<uintptr_t>((b_rows - 1) * ldb + width) * size;
-    return a_rows > 0 && b_rows > 0 && width > 0 && x < y + ys && y < x + xs;
-}
 
 }  // namespace
 
@@ -190,7 +185,8 @@ int launch_expert_gather(int type, const void* x, long long ldx, long long token
     if (tokens == 0 || n_slots == 0 || width == 0) return 0;
     if (rows == nullptr || !aligned4(rows)) return fail(1, "%s: rows must be a 4-byte aligned device pointer", who);
     const int size = type == kTypeF32 ? 4 : 2;
-    if (rows_overlap(x, tokens, ldx, out, n_slots, ldo, width, size)) return fail(1, "%s: x and the result overlap", who);
+    if (outputs_overlap({matrix_span(out, n_slots, width, ldo, size)}, {matrix_span(x, tokens, width, ldx, size), entries_span(rows, n_slots)}))
+        return fail(1, "%s: the result overlaps an input", who);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T>::N)));
@@ -210,7 +206,9 @@ int launch_expert_sum(int type, const void* y, long long ldy, long long n_slots,
     if (slots == nullptr || !aligned4(slots) || !aligned4(weights)) return fail(1, "%s: slots and weights must be 4-byte aligned device pointers", who);
     if (out == nullptr || ldo < width) return fail(1, "%s: null result or a row stride shorter than its row", who);
     const int size = type == kTypeF32 ? 4 : 2;
-    if (rows_overlap(y, n_slots, ldy, out, tokens, ldo, width, size)) return fail(1, "%s: y and the result overlap", who);
+    if (outputs_overlap({matrix_span(out, tokens, width, ldo, size)},
+                        {matrix_span(y, n_slots, width, ldy, size), entries_span(weights, tokens * k), entries_span(slots, tokens * k)}))
+        return fail(1, "%s: the result overlaps an input", who);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const int parts = static_cast<int>(ceil_div(width, static_cast<long long>(kWave * Packet<T>::N)));
@@ -236,9 +234,11 @@ int launch_expert_sum_backward(int type, const void* dout, long long ldd, const 
     if (slots == nullptr || weights == nullptr || dw == nullptr || !aligned4(slots) || !aligned4(weights) || !aligned4(dw))
         return fail(1, "%s: slots, weights and their gradient must be 4-byte aligned device pointers", who);
     const int size = type == kTypeF32 ? 4 : 2;
-    if (rows_overlap(y, n_slots, ldy, dy, n_slots, lddy, width, size) || rows_overlap(dout, tokens, ldd, dy, n_slots, lddy, width, size))
-        return fail(1, "%s: the gradient of y overlaps an input", who);
     const long long entries = tokens * k;
+    if (outputs_overlap({matrix_span(dy, n_slots, width, lddy, size), entries_span(dw, entries)},
+                        {matrix_span(dout, tokens, width, ldd, size), matrix_span(y, n_slots, width, ldy, size), entries_span(weights, entries),
+                         entries_span(slots, entries)}))
+        return fail(1, "%s: a result overlaps an input or the other result", who);
     const bool stream = streams(n_slots, width, size);
     const long long blocks = ceil_div(entries, static_cast<long long>(stream ? kRowsWaves / 2 : kRowsWaves));
     if (!launchable(blocks, kRowsBlock)) return fail(1, "%s: too much work for one launch", who);

@@ -952,15 +952,6 @@ int run(GroupedProblem g, const char* who, hipStream_t s) {
     return check_launch("gemm_grouped_kernel");
 }
 
-// The bytes from p that a rows x cols matrix of row stride ld occupies.
-uintptr_t span_bytes(long long rows, long long cols, long long ld, int size) {
-    return rows <= 0 || cols <= 0 ? 0 : static_cast<uintptr_t>((rows - 1) * ld + cols) * size;
-}
-bool overlap(const void* a, uintptr_t a_bytes, const void* b, uintptr_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + b_bytes && y < x + a_bytes;
-}
-
 }  // namespace
 
 int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int K, const uint16_t* first, long long ld_first,
@@ -988,11 +979,12 @@ int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int
     if (offsets == nullptr || out == nullptr || (depth > 0 && (first == nullptr || second == nullptr))) return fail(1, "%s: null pointer", who);
     if (!aligned2(first) || !aligned2(second) || !aligned4(offsets) || !(size == 4 ? aligned4(out) : aligned2(out)))
         return fail(1, "%s: misaligned pointer", who);
-    const uintptr_t group_bytes = (static_cast<uintptr_t>(groups - 1) * group_stride) * (grad_b ? size : 2) + span_bytes(N, K, ld_group, grad_b ? size : 2);
-    const uintptr_t out_bytes = grad_b ? group_bytes : span_bytes(rows, out_cols, ld_out, size);
-    if (overlap(out, out_bytes, first, span_bytes(rows, first_cols, ld_first, 2)) ||
-        overlap(out, out_bytes, second, grad_b ? span_bytes(rows, K, ld_second, 2) : group_bytes) ||
-        overlap(out, out_bytes, offsets, (static_cast<uintptr_t>(groups) + 1) * 4))
+    const int group_size = grad_b ? size : 2;
+    Span matrices = matrix_span(grad_b ? out : second, N, K, ld_group, group_size);
+    if (matrices.bytes != 0) matrices.bytes += static_cast<uintptr_t>(groups - 1) * group_stride * group_size;
+    if (outputs_overlap({grad_b ? matrices : matrix_span(out, rows, out_cols, ld_out, size)},
+                        {matrix_span(first, rows, first_cols, ld_first, 2), grad_b ? matrix_span(second, rows, K, ld_second, 2) : matrices,
+                         entries_span(offsets, groups + 1ll)}))
         return fail(1, "%s: the output overlaps an input", who);
 
     GroupedProblem g{};

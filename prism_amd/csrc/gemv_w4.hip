@@ -343,12 +343,11 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
     p.groups = groups; p.rows = static_cast<int>(rows); p.N = N; p.K = K; p.G = group_size;
     p.n_groups = ceil_div(K, group_size);
     p.s_stride = static_cast<long long>(N) * p.n_groups;
-    const uintptr_t yb = reinterpret_cast<uintptr_t>(y), ye = yb + static_cast<uintptr_t>((rows - 1) * ldy + N) * size;
-    auto meets = [&](const void* a, uintptr_t bytes) { const uintptr_t b = reinterpret_cast<uintptr_t>(a); return a != nullptr && b < ye && yb < b + bytes; };
-    if (meets(x, static_cast<uintptr_t>((rows - 1) * ldx + K) * 2) ||
-        meets(q, static_cast<uintptr_t>(groups - 1) * q_stride + static_cast<uintptr_t>(N - 1) * ldq + (K + 1) / 2) ||
-        meets(scales, static_cast<uintptr_t>(groups) * p.s_stride * 2) || meets(zeros, static_cast<uintptr_t>(groups) * p.s_stride) ||
-        meets(offsets, (static_cast<uintptr_t>(groups) + 1) * 4))
+    Span matrices = matrix_span(q, N, (K + 1) / 2, ldq, 1);
+    if (matrices.bytes != 0) matrices.bytes += static_cast<uintptr_t>(groups - 1) * q_stride;
+    const uintptr_t scale_count = static_cast<uintptr_t>(groups) * p.s_stride;
+    if (outputs_overlap({matrix_span(y, rows, N, ldy, size)}, {matrix_span(x, rows, K, ldx, 2), matrices, Span{scales, scale_count * 2}, Span{zeros, scale_count},
+                                                               entries_span(offsets, groups + 1ll)}))
         return fail(1, "%s: the output overlaps an input", who);
     const long long row_tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16) : ceil_div(rows, 16ll);
     const long long busy = offsets != nullptr ? busy_row_tiles(rows, groups, row_tiles) : row_tiles;

@@ -511,6 +511,12 @@ int check_plan(const char* who, const int32_t* chosen, long long tokens, int k, 
     return 0;
 }
 
+Span logits_span(const void* at, int type, long long tokens, int experts, long long ld) { return matrix_span(at, tokens, experts, ld, type == kTypeF32 ? 4 : 2); }
+// Of a workspace only what the plan needs.
+Span plan_workspace_span(const void* ws, long long tokens, int k, int experts) {
+    return {ws, one_run(tokens * k, experts) ? 0 : expert_plan_workspace_bytes(tokens, k, experts)};
+}
+
 // The router's kernels for a logit type, a number of experts and an alignment: f(T, values of a lane, values of an access).
 template <typename F>
 int with_logits(int type, const void* logits, long long ld, int experts, F&& f) {
@@ -541,8 +547,12 @@ size_t expert_plan_workspace_bytes(long long tokens, int k, int experts) {
 
 int launch_expert_plan(const int32_t* chosen, long long tokens, int k, int experts, int32_t* offsets, int32_t* rows, int32_t* slots, void* ws,
                        size_t ws_bytes, hipStream_t s) {
-    if (int rc = check_plan("prism_expert_plan", chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes)) return rc;
+    const char* who = "prism_expert_plan";
+    if (int rc = check_plan(who, chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes)) return rc;
     const int entries = static_cast<int>(tokens * k);
+    if (outputs_overlap({entries_span(offsets, experts + 1ll), entries_span(rows, entries), entries_span(slots, entries), plan_workspace_span(ws, tokens, k, experts)},
+                        {entries_span(chosen, entries)}))
+        return fail(1, "%s: a result or the workspace overlaps the experts or another one", who);
     if (one_run(entries, experts)) {
         plan_small_kernel<<<dim3(1), dim3(kRunWaves * kWave), run_lds(experts), s>>>(chosen, entries, experts, bits_of(experts), offsets, rows, slots);
         return check_launch("plan_small_kernel");
@@ -568,8 +578,11 @@ int check_route_call(const char* who, int type, const void* logits, long long ld
 
 int launch_route_topk(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,
                       hipStream_t s) {
-    if (int rc = check_route_call("prism_route_topk", type, logits, ld, tokens, experts, k, weights, chosen)) return rc;
+    const char* who = "prism_route_topk";
+    if (int rc = check_route_call(who, type, logits, ld, tokens, experts, k, weights, chosen)) return rc;
     if (tokens == 0) return 0;
+    if (outputs_overlap({entries_span(weights, tokens * k), entries_span(chosen, tokens * k)}, {logits_span(logits, type, tokens, experts, ld)}))
+        return fail(1, "%s: a result overlaps the logits or the other result", who);
     return with_logits(type, logits, ld, experts, [&](auto t, auto values, auto pack) {
         using T = decltype(t);
         constexpr int V = decltype(values)::value, P = decltype(pack)::value;
@@ -586,6 +599,10 @@ int launch_route_plan(int type, const void* logits, long long ld, long long toke
     if (int rc = check_route_call(who, type, logits, ld, tokens, experts, k, weights, chosen)) return rc;
     if (int rc = check_plan(who, chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes)) return rc;
     if (tokens == 0) return launch_expert_plan(chosen, tokens, k, experts, offsets, rows, slots, ws, ws_bytes, s);
+    if (outputs_overlap({entries_span(weights, tokens * k), entries_span(chosen, tokens * k), entries_span(offsets, experts + 1ll), entries_span(rows, tokens * k),
+                         entries_span(slots, tokens * k), plan_workspace_span(ws, tokens, k, experts)},
+                        {logits_span(logits, type, tokens, experts, ld)}))
+        return fail(1, "%s: a result or the workspace overlaps the logits or another one", who);
     constexpr int TOKENS = kRunWaves * kWave / kLanes;  // of a workgroup
     if (tokens > TOKENS && one_run(tokens * k, experts)) {  // too many for one workgroup's router, and no workspace to count in
         if (int rc = launch_route_topk(type, logits, ld, tokens, experts, k, renormalise, weights, chosen, s)) return rc;
@@ -618,8 +635,9 @@ int launch_route_backward(int type, const float* grad, const void* logits, long 
     const unsigned size = type == kTypeF32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(out) % size != 0 || !aligned4(grad)) return fail(1, "%s: misaligned pointer", who);
     if (tokens > 1 && ldo < experts) return fail(1, "%s: a row stride is shorter than its row (%d)", who, experts);
-    const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(out);
-    if (a < b + ((tokens - 1) * ldo + experts) * size && b < a + ((tokens - 1) * ld + experts) * size) return fail(1, "%s: the result overlaps the logits", who);
+    if (outputs_overlap({logits_span(out, type, tokens, experts, ldo)},
+                        {logits_span(logits, type, tokens, experts, ld), entries_span(grad, tokens * k), entries_span(weights, tokens * k), entries_span(chosen, tokens * k)}))
+        return fail(1, "%s: the result overlaps an input", who);
     const dim3 grid(static_cast<unsigned>(ceil_div(tokens, static_cast<long long>(kRouteBlock / kLanes))));
     auto go = [&](auto t, auto pack) {
         using T = decltype(t);

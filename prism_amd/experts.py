@@ -9,7 +9,8 @@
 and the gradient of each as a call of its own. Like the calls in ops.py they run on torch's current stream of the
 tensors' device, are asynchronous, take their outputs as arguments or allocate them, and raise ValueError / TypeError
 for arguments they cannot work on. Matrices are row-major with any distance between rows (the last dimension must be
-contiguous). Nothing is copied to the host: the group offsets stay on the device.
+contiguous). An output that overlaps an input or another output, from a matrix' first element to its last (columns of one
+buffer do), is refused. Nothing is copied to the host: the group offsets stay on the device.
 
 One layer, forward:
 
