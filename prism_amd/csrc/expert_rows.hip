@@ -204,8 +204,10 @@ int launch_expert_sum(int type, const void* y, long long ldy, long long n_slots,
     if (int rc = check_rows(who, type, tokens, k, n_slots, width, {y, out}, {ldy, ldo})) return rc;
     if (tokens == 0 || width == 0) return 0;
     if (slots == nullptr || !aligned4(slots) || !aligned4(weights)) return fail(1, "%s: slots and weights must be 4-byte aligned device pointers", who);
-    if (out == nullptr || ldo < width) return fail(1, "%s: null result or a row stride shorter than its row", who);
     const int size = type == kTypeF32 ? 4 : 2;
+    // Written also where there are no slots, which check_rows takes for an empty call.
+    if (out == nullptr || ldo < width) return fail(1, "%s: null result or a row stride shorter than its row", who);
+    if (reinterpret_cast<uintptr_t>(out) % size != 0) return fail(1, "%s: misaligned pointer", who);
     if (outputs_overlap({matrix_span(out, tokens, width, ldo, size)},
                         {matrix_span(y, n_slots, width, ldy, size), entries_span(weights, tokens * k), entries_span(slots, tokens * k)}))
         return fail(1, "%s: the result overlaps an input", who);

@@ -77,3 +77,10 @@ def test_products(lib):
     w = {"x": at(0), "q": at(1), "scales": at(2), "zeros": at(3), "offsets": at(4), "y": at(5)}
     overlaps(lib, lambda o: lib.prism_gemv_w4(G, R, N, K, o["x"], K, o["q"], K // 2, N * K // 2, o["scales"], o["zeros"], 32, o["offsets"], o["y"], N, 0, None), w,
              [("y", "x", a), ("y", "q", G * N * K // 2), ("y", "scales", 2 * G * N * K // 32), ("y", "zeros", G * N * K // 32), ("y", "offsets", 4 * (G + 1))])
+
+
+def test_a_sum_without_slots_checks_its_result(lib):
+    """It is written (zeros) though there is nothing to add up."""
+    for out, ld, text in ((at(3) + 1, 8, "misaligned"), (at(3), 7, "row stride"), (None, 8, "null")):
+        assert lib.prism_expert_combine(None, 1, 8, 0, None, at(2), 4, 2, out, ld, 8, None) == 1
+        assert text in lib.prism_last_error_string().decode()
