@@ -14,8 +14,6 @@ struct GroupTile {
     int group;    // -1: there is no such tile
     int row0;     // the tile's first row
     int row_end;  // one past the group's last row
-    int tiles;    // tiles of the group
-    int index;    // this tile's number within the group
 };
 
 __device__ __forceinline__ int clamp_offset(int v, int rows) { return v < 0 ? 0 : (v > rows ? rows : v); }
@@ -30,9 +28,9 @@ __device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
 }
 
 // Tile number `tile` of the row tiles of all groups, in group order, each group cut into tiles of `tile_rows` rows.
-// Called by whole wavefronts; the result is wave-uniform. `total` (if not null) gets the number of tiles when the
-// tile does not exist.
-__device__ __forceinline__ GroupTile find_group_tile(const int32_t* offsets, int groups, int rows, int tile, int tile_rows, int* total = nullptr) {
+// Called by whole wavefronts; the result is wave-uniform. The sums stay below 2^31 whatever the table holds: a launch has at
+// most 2^24 row tiles, no group has more tiles than that, and the search ends in the 64 groups that pass `tile`.
+__device__ __forceinline__ GroupTile find_group_tile(const int32_t* offsets, int groups, int rows, int tile, int tile_rows) {
     const int lane = threadIdx.x & (kWave - 1);
     int before = 0;
     for (int base = 0; base < groups; base += kWave) {
@@ -49,17 +47,14 @@ __device__ __forceinline__ GroupTile find_group_tile(const int32_t* offsets, int
             const int src = __builtin_ctzll(mask);
             GroupTile t;
             t.group = __builtin_amdgcn_readfirstlane(base + src);
-            t.tiles = __builtin_amdgcn_readlane(tiles, src);
-            t.index = tile - (__builtin_amdgcn_readlane(upto, src) - t.tiles);
-            t.row0 = __builtin_amdgcn_readlane(lo, src) + t.index * tile_rows;
+            const int index = tile - (__builtin_amdgcn_readlane(upto, src) - __builtin_amdgcn_readlane(tiles, src));  // within the group
+            t.row0 = __builtin_amdgcn_readlane(lo, src) + index * tile_rows;
             t.row_end = __builtin_amdgcn_readlane(hi, src);
-            if (t.index < 0 || t.row0 >= t.row_end) t.group = -1;
             return t;
         }
         before = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
-    if (total != nullptr) *total = before;
-    return GroupTile{-1, 0, 0, 0, 0};
+    return GroupTile{-1, 0, 0};
 }
 
 // The most row tiles that groups of together `rows` rows can have: a group wastes less than one tile, and a tile has
