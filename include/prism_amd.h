@@ -499,6 +499,18 @@ int prism_gemm_bf16_grouped_grad_b(int groups, int64_t rows, int N, int K, const
                                    void* dB, int64_t ldb, int64_t group_stride, int b_type, void* stream);
 
 /*
+ * Which kernel the three products above take for these sizes on the current
+ * device, given contiguous operands with 16-byte aligned bases: *tile_rows =
+ * 16, 128 or 256, the rows of its tiles, and *stages = 0, 4 or 2 (128 rows) or
+ * 2, the stages of the ring in LDS that it loads ahead; both 0 for an empty
+ * call. Either pointer may be NULL. Operands of other alignments take tiles of
+ * 16 or 128 rows. Lets a harness or test assert which kernel it measures.
+ */
+enum { PRISM_GROUPED_FORWARD = 0, PRISM_GROUPED_GRAD_A = 1, PRISM_GROUPED_GRAD_B = 2 };
+int prism_gemm_bf16_grouped_plan(int form, int groups, int64_t rows, int N, int K, int out_type,
+                                 int* tile_rows, int* stages);
+
+/*
  * A few rows times weights held in 4 bits: y[r][n] = sum_k x[r][k] scales[n][k
  * / group_size] (q[n][k] - zeros[n][k / group_size]) for the rows of group g
  * and its matrix. x: rows x K bf16, any finite numbers (an infinity gives

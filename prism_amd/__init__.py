@@ -39,6 +39,7 @@ from .experts import (  # noqa: F401
     gemm_bf16_grouped,
     gemm_bf16_grouped_grad_a,
     gemm_bf16_grouped_grad_b,
+    gemm_bf16_grouped_plan,
     gemv_w4,
     route_topk,
     route_topk_backward,

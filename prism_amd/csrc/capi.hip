@@ -196,6 +196,13 @@ int prism_gemm_bf16_grouped_grad_b(int groups, int64_t rows, int N, int K, const
                                static_cast<hipStream_t>(stream));
 }
 
+static_assert(PRISM_GROUPED_FORWARD == static_cast<int>(GroupedForm::kForward) && PRISM_GROUPED_GRAD_A == static_cast<int>(GroupedForm::kGradA) &&
+                  PRISM_GROUPED_GRAD_B == static_cast<int>(GroupedForm::kGradB), "include/prism_amd.h and common.h disagree");
+
+int prism_gemm_bf16_grouped_plan(int form, int groups, int64_t rows, int N, int K, int out_type, int* tile_rows, int* stages) {
+    return gemm_grouped_plan(form, groups, rows, N, K, out_type, tile_rows, stages);
+}
+
 int prism_gemv_w4(int groups, int64_t rows, int N, int K, const uint16_t* x, int64_t ldx, const uint8_t* q, int64_t ldq, int64_t group_stride,
                   const uint16_t* scales, const uint8_t* zeros, int group_size, const int32_t* offsets, void* y, int64_t ldy, int y_type, void* stream) {
     return launch_gemv_w4(groups, rows, N, K, x, ldx, q, ldq, group_stride, scales, zeros, group_size, offsets, y, ldy, y_type,

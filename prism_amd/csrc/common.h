@@ -124,6 +124,8 @@ enum class GroupedForm { kForward, kGradA, kGradB };
 int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int K, const uint16_t* first, long long ld_first,
                         const uint16_t* second, long long ld_second, long long group_stride, const int32_t* offsets, void* out,
                         long long ld_out, int out_type, hipStream_t s);
+// Which kernel a product of contiguous operands takes: the rows of its tiles and the stages of its ring.
+int gemm_grouped_plan(int form, int groups, long long rows, int N, int K, int out_type, int* tile_rows, int* stages);
 int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, long long ldx, const uint8_t* q, long long ldq, long long q_stride,
                    const uint16_t* scales, const uint8_t* zeros, int group_size, const int32_t* offsets, void* y, long long ldy, int out_type, hipStream_t s);
 int launch_route_topk(int type, const void* logits, long long ld, long long tokens, int experts, int k, int renormalise, float* weights, int32_t* chosen,

@@ -921,16 +921,28 @@ Kernel choose_kernel(const GroupedProblem& g, int out_size, bool can_few, bool c
     return single <= pairs ? Kernel::kGeneral : Kernel::kGeneralPairs;
 }
 
+// Rows of a tile of 32-bit offsets from each other.
+bool near_rows(const GroupedProblem& g) { return g.ldp < (1 << 21) && g.ldq < (1 << 21); }
+// 16 B chunks are whole or absent throughout (bases, strides and the extents along memory in multiples of 8 elements), with
+// 32-bit offsets inside a tile. What is not runs on the general kernel, or on the one for few rows.
+template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C>
+bool whole_chunks(const GroupedProblem& g) {
+    const int p_along = P_TURNED ? g.out_rows : g.depth, q_along = Q_TURNED ? g.cols : g.depth;
+    return aligned16(g.P) && aligned16(g.Q) && g.ldp % 8 == 0 && g.ldq % 8 == 0 && (RAGGED_C || g.group_stride % 8 == 0) && p_along % 8 == 0 &&
+           q_along % 8 == 0 && near_rows(g);
+}
+template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C>
+Kernel choose_kernel(const GroupedProblem& g, int out_size) {
+    return choose_kernel<RAGGED_C>(g, out_size, !P_TURNED && !Q_TURNED,
+                                   whole_chunks<P_TURNED, Q_TURNED, RAGGED_C>(g) && g.groups <= kBigGroups && cu_count() >= 8);
+}
+
 template <bool P_TURNED, bool Q_TURNED, bool RAGGED_C, typename OutT>
 int run(GroupedProblem g, const char* who, hipStream_t s) {
     constexpr bool FORWARD = !P_TURNED && !Q_TURNED;
-    // Aligned: 16 B chunks are whole or absent throughout (bases, strides and the extents along memory in multiples of 8
-    // elements), with 32-bit offsets inside a tile. What is not runs on the general kernel, or on the one for few rows.
-    g.near = g.ldp < (1 << 21) && g.ldq < (1 << 21);
-    const int p_along = P_TURNED ? g.out_rows : g.depth, q_along = Q_TURNED ? g.cols : g.depth;
-    const bool aligned = aligned16(g.P) && aligned16(g.Q) && g.ldp % 8 == 0 && g.ldq % 8 == 0 && (RAGGED_C || g.group_stride % 8 == 0) &&
-                         p_along % 8 == 0 && q_along % 8 == 0 && g.near;
-    const Kernel kernel = choose_kernel<RAGGED_C>(g, static_cast<int>(sizeof(OutT)), FORWARD, aligned && g.groups <= kBigGroups && cu_count() >= 8);
+    g.near = near_rows(g);
+    const bool aligned = whole_chunks<P_TURNED, Q_TURNED, RAGGED_C>(g);
+    const Kernel kernel = choose_kernel<P_TURNED, Q_TURNED, RAGGED_C>(g, static_cast<int>(sizeof(OutT)));
     if constexpr (FORWARD)
         if (kernel == Kernel::kFew) return run_few<OutT>(g, who, s);
     const int edge = kernel == Kernel::kBig ? 256 : 128;
@@ -954,16 +966,43 @@ int run(GroupedProblem g, const char* who, hipStream_t s) {
 
 }  // namespace
 
-int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int K, const uint16_t* first, long long ld_first,
-                        const uint16_t* second, long long ld_second, long long group_stride, const int32_t* offsets, void* out,
-                        long long ld_out, int out_type, hipStream_t s) {
-    const char* who = form == GroupedForm::kForward ? "prism_gemm_bf16_grouped"
-                      : form == GroupedForm::kGradA ? "prism_gemm_bf16_grouped_grad_a" : "prism_gemm_bf16_grouped_grad_b";
+static int check_grouped_sizes(const char* who, int groups, long long rows, int N, int K, int out_type) {
     if (groups < 0 || rows < 0 || N < 0 || K < 0) return fail(1, "%s: negative dimension (%d groups, %lld rows, N=%d, K=%d)", who, groups, rows, N, K);
     if (rows > 0x7fffffffll - 256) return fail(1, "%s: %lld rows, at most 2^31 - 257 are supported", who, rows);
     if (groups > 0x7fffffff - 4096 || N > 0x7fffffff - 4096 || K > 0x7fffffff - 4096)
         return fail(1, "%s: %d groups, N=%d, K=%d: at most 2^31 - 4097 are supported", who, groups, N, K);
     if (out_type != kTypeF32 && out_type != kTypeBf16) return fail(1, "%s: unknown output type %d", who, out_type);
+    return 0;
+}
+
+int gemm_grouped_plan(int form, int groups, long long rows, int N, int K, int out_type, int* tile_rows, int* stages) {
+    const char* who = "prism_gemm_bf16_grouped_plan";
+    if (form < 0 || form > static_cast<int>(GroupedForm::kGradB)) return fail(1, "%s: unknown form %d", who, form);
+    if (int rc = check_grouped_sizes(who, groups, rows, N, K, out_type)) return rc;
+    const GroupedForm f = static_cast<GroupedForm>(form);
+    const bool empty = groups == 0 || (f == GroupedForm::kGradB ? N == 0 || K == 0 : rows == 0 || (f == GroupedForm::kForward ? N : K) == 0);
+    GroupedProblem g{};  // contiguous, bases at address 0
+    g.ldp = f == GroupedForm::kForward ? K : N;
+    g.ldq = K;
+    g.group_stride = static_cast<long long>(N) * K;
+    g.groups = groups; g.rows = static_cast<int>(rows); g.cols = f == GroupedForm::kForward ? N : K;
+    g.depth = f == GroupedForm::kForward ? K : (f == GroupedForm::kGradA ? N : 0); g.out_rows = N;
+    const int size = out_type == kTypeF32 ? 4 : 2;
+    Kernel kernel = Kernel::kFew;
+    if (!empty)
+        kernel = f == GroupedForm::kForward ? choose_kernel<false, false, false>(g, size)
+                 : f == GroupedForm::kGradA ? choose_kernel<false, true, false>(g, size) : choose_kernel<true, true, true>(g, size);
+    if (tile_rows) *tile_rows = empty ? 0 : (kernel == Kernel::kFew ? 16 : (kernel == Kernel::kBig ? 256 : 128));
+    if (stages) *stages = empty || kernel == Kernel::kFew ? 0 : (kernel == Kernel::kGeneral ? 4 : 2);
+    return 0;
+}
+
+int launch_gemm_grouped(GroupedForm form, int groups, long long rows, int N, int K, const uint16_t* first, long long ld_first,
+                        const uint16_t* second, long long ld_second, long long group_stride, const int32_t* offsets, void* out,
+                        long long ld_out, int out_type, hipStream_t s) {
+    const char* who = form == GroupedForm::kForward ? "prism_gemm_bf16_grouped"
+                      : form == GroupedForm::kGradA ? "prism_gemm_bf16_grouped_grad_a" : "prism_gemm_bf16_grouped_grad_b";
+    if (int rc = check_grouped_sizes(who, groups, rows, N, K, out_type)) return rc;
     const int size = out_type == kTypeF32 ? 4 : 2;
     const bool grad_b = form == GroupedForm::kGradB;
     // Row lengths of the operands, and the group matrices' shape (always N x K).

@@ -338,6 +338,23 @@ def gemm_bf16_grouped_grad_b(dD: "torch.Tensor", A: "torch.Tensor", offsets: "to
     return dB
 
 
+_FORMS = {"forward": 0, "grad_a": 1, "grad_b": 2}  # PRISM_GROUPED_* of include/prism_amd.h
+
+
+def gemm_bf16_grouped_plan(form: str, groups: int, rows: int, N: int, K: int, out_dtype: "torch.dtype" = torch.float32) -> Tuple[int, int]:
+    """(rows of a tile, stages of its ring in LDS) of the kernel that a grouped product ("forward", "grad_a" or "grad_b") of
+    contiguous, 16-byte aligned operands takes: (16, 0), (128, 4), (128, 2) or (256, 2); (0, 0) for an empty call."""
+    import ctypes
+    if form not in _FORMS:
+        raise ValueError(f"gemm_bf16_grouped_plan: form {form!r} not in {tuple(_FORMS)}")
+    if out_dtype not in _TYPES:
+        raise TypeError(f"out_dtype: {out_dtype} not in {tuple(_TYPES)}")
+    tile, stages = ctypes.c_int(0), ctypes.c_int(0)
+    _check(_lib.load().prism_gemm_bf16_grouped_plan(_FORMS[form], _int(groups, "groups"), _int(rows, "rows"), _int(N, "N"), _int(K, "K"), _TYPES[out_dtype],
+                                                    ctypes.byref(tile), ctypes.byref(stages)), "gemm_bf16_grouped_plan")
+    return tile.value, stages.value
+
+
 def gemv_w4(x: "torch.Tensor", q: "torch.Tensor", scales: "torch.Tensor", group_size: int, zeros: Optional["torch.Tensor"] = None,
             offsets: Optional["torch.Tensor"] = None, out: Optional["torch.Tensor"] = None,
             out_dtype: "torch.dtype" = torch.bfloat16) -> "torch.Tensor":

@@ -2,10 +2,12 @@
 
 Tolerances as in test_gpu_experts.py; products of small whole numbers are exact and compared bit by bit.
 """
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_experts import DEV, near, normal
+from test_experts_plan import KERNELS
+from test_gpu_experts import DEV, near, normal, table
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +53,35 @@ def test_w4_of_rows_of_any_size(prism, rows, k, group, power):
     v = w4_values(q, k)
     out = prism.gemv_w4(x, q, s, group, out_dtype=torch.float32)
     near(out, x.double() @ (v - 8).T * 2.0 ** -power, x.double().abs() @ (40 + v).T * 2.0 ** -power, 128 + k // 32 + 16)
+
+
+# ---------------------------------------------------------------------------------------------------------- products --
+
+@pytest.mark.parametrize("form,groups,rows,n,k,dtype,kernel", KERNELS)
+def test_every_kernel_of_the_products_on_whole_numbers(prism, form, groups, rows, n, k, dtype, kernel):
+    """Sums below 2^24 of whole numbers are exact in fp32 in any order, so a result is the exact sum, rounded once: the same
+    bits as the library product of each group. One group is empty, the others' sizes are uneven."""
+    assert prism.gemm_bf16_grouped_plan(form, groups, rows, n, k, dtype) == kernel
+    rng = np.random.default_rng(rows)
+    sizes = rng.multinomial(rows, [0.0] + [1 / (groups - 1)] * (groups - 1))
+    offsets, ends = table(sizes), np.concatenate([[0], np.cumsum(sizes)]).tolist()
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    whole = lambda *shape: torch.randint(-3, 4, shape, generator=gen, device=DEV, dtype=torch.int8).bfloat16()  # noqa: E731
+    a = whole(rows, k) if form != "grad_a" else None
+    d = whole(rows, n) if form != "forward" else None
+    b = whole(groups, n, k) if form != "grad_b" else None
+    if form == "forward":
+        out = prism.gemm_bf16_grouped(a, b, offsets, out_dtype=dtype)
+    elif form == "grad_a":
+        out = prism.gemm_bf16_grouped_grad_a(d, b, offsets, out_dtype=dtype)
+    else:
+        out = prism.gemm_bf16_grouped_grad_b(d, a, offsets, out_dtype=dtype)
+    for g in range(groups):
+        lo, hi = ends[g], ends[g + 1]
+        if form == "forward":
+            got, want = out[lo:hi], a[lo:hi].float() @ b[g].float().t()
+        elif form == "grad_a":
+            got, want = out[lo:hi], d[lo:hi].float() @ b[g].float()
+        else:
+            got, want = out[g], d[lo:hi].float().t() @ a[lo:hi].float()
+        assert torch.equal(got, want.to(dtype)), f"group {g} of {hi - lo} rows"
