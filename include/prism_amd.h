@@ -406,7 +406,8 @@ enum { PRISM_TYPE_F32 = 0, PRISM_TYPE_BF16 = 1 };
  * logit (equal ones: the lower index; NaN counts as the largest; -inf is never
  * chosen: -1 where nothing is left) and weights[t * k + j] =
  * exp(z_j - z_0) / sum, summed over the chosen ones (renormalise != 0) or over
- * all logits of the token; 0 for expert -1. At most 1024 experts, k <= 32.
+ * all logits of the token; 0 for expert -1. A token whose largest logit is NaN
+ * or +inf has NaN among its weights. At most 1024 experts, k <= 32.
  */
 int prism_route_topk(const void* logits, int type, int64_t ld, int64_t tokens, int experts, int k,
                      int renormalise, float* weights, int32_t* chosen, void* stream);

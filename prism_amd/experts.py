@@ -10,7 +10,9 @@ and the gradient of each as a call of its own. Like the calls in ops.py they run
 tensors' device, are asynchronous, take their outputs as arguments or allocate them, and raise ValueError / TypeError
 for arguments they cannot work on. Matrices are row-major with any distance between rows (the last dimension must be
 contiguous). An output that overlaps an input or another output, from a matrix' first element to its last (columns of one
-buffer do), is refused. Nothing is copied to the host: the group offsets stay on the device.
+buffer do), is refused. Nothing is copied to the host: the group offsets stay on the device. Nothing is recorded for
+autograd: results of inputs that require gradients do not; a torch.autograd.Function around a call and its gradient call
+records them.
 
 One layer, forward:
 
@@ -137,7 +139,7 @@ def route_topk(logits: "torch.Tensor", k: int, renormalise: bool = True, out: Op
 
     logits: [T, E] fp32 or bf16, E <= 1024, k <= min(E, 32). Equal logits go to the lower index, -inf is never chosen
     (a token with fewer than k others gets expert -1, weight 0), NaN counts as the largest. weights: the softmax over the
-    chosen logits (renormalise) or over all of them. The plan is expert_plan's. out: a Routing (or five tensors in its
+    chosen logits (renormalise) or over all of them; a token whose largest logit is NaN or +inf has NaN among them. The plan is expert_plan's. out: a Routing (or five tensors in its
     order) to write into.
     """
     ld = _matrix(logits, _TYPES, "logits")

@@ -85,3 +85,45 @@ def test_every_kernel_of_the_products_on_whole_numbers(prism, form, groups, rows
         else:
             got, want = out[g], d[lo:hi].float().t() @ a[lo:hi].float()
         assert torch.equal(got, want.to(dtype)), f"group {g} of {hi - lo} rows"
+
+
+class GroupedProduct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, b, offsets):
+        import prism_amd as prism
+        ctx.save_for_backward(a, b, offsets)
+        return prism.gemm_bf16_grouped(a, b, offsets, out_dtype=torch.bfloat16)
+
+    @staticmethod
+    def backward(ctx, grad):
+        import prism_amd as prism
+        a, b, offsets = ctx.saved_tensors
+        grad = grad.contiguous()
+        return (prism.gemm_bf16_grouped_grad_a(grad, b, offsets, out_dtype=torch.bfloat16),
+                prism.gemm_bf16_grouped_grad_b(grad, a, offsets, out_dtype=torch.bfloat16), None)
+
+
+def test_gradients_are_recorded_by_a_function_around_the_calls_and_by_nothing_else(prism):
+    """Whole numbers: every sum is exact and rounded once, as in the reference product by product."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    a, b, up = (torch.randint(-3, 4, s, generator=gen, device=DEV).bfloat16() for s in ((90, 64), (3, 48, 64), (90, 48)))
+    a.requires_grad_()
+    b.requires_grad_()
+    sizes, ends = [30, 0, 60], [0, 30, 30, 90]
+    assert not prism.gemm_bf16_grouped(a, b, table(sizes)).requires_grad
+    GroupedProduct.apply(a, b, table(sizes)).backward(up)
+    for g in range(3):
+        rows = slice(ends[g], ends[g + 1])
+        assert torch.equal(a.grad[rows], (up[rows].float() @ b[g].detach().float()).bfloat16())
+        assert torch.equal(b.grad[g], (up[rows].float().t() @ a[rows].detach().float()).bfloat16())
+
+
+def test_weights_of_a_token_whose_largest_logit_is_not_a_number(prism):
+    """As documented, for both types and both sums: the choice is made, NaN is among the weights of that token and of no other."""
+    z = normal(3, 5, 40)
+    z[1, 7], z[2, 9], z[3, 3:5] = float("nan"), float("inf"), float("inf")
+    for dtype in (torch.float32, torch.bfloat16):
+        for renormalise in (True, False):
+            r = prism.route_topk(z.to(dtype), 4, renormalise=renormalise)
+            assert r.experts[1:4, 0].tolist() == [7, 9, 3] and int(r.experts[3, 1]) == 4
+            assert r.weights.isnan().any(1).tolist() == [False, True, True, True, False]
