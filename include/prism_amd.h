@@ -520,8 +520,8 @@ int prism_gemm_bf16_grouped_plan(int form, int groups, int64_t rows, int N, int 
  * the low nibble; ldq and group_stride in bytes. scales (bf16) and zeros (uint8, NULL:
  * 8 throughout): groups x N x ceil(K / group_size), contiguous; group_size a
  * multiple of 32. offsets may be NULL for one matrix: all rows use it. y: rows
- * x N of y_type. Made for up to 16 rows a group; more are right, and fetch the
- * weights once per 16 rows (from the L2 after the first).
+ * x N of y_type. Made for few rows a group; any number is right, and every 16
+ * rows unpack the weights again.
  */
 int prism_gemv_w4(int groups, int64_t rows, int N, int K, const uint16_t* x, int64_t ldx,
                   const uint8_t* q, int64_t ldq, int64_t group_stride, const uint16_t* scales,

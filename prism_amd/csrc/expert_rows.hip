@@ -6,8 +6,10 @@
 // Unused slots are left as they are, a token without experts gets zeros. Sums run over j (and, in the dot products,
 // over the row) in 32 bits and in a fixed order: the same bits on every run.
 //
-// HBM-bound: every row is read once and written once. 8192 tokens x 8 x 4096 bf16, a random choice of 64 experts: gather 139 us
-// (604 MB, 4.3 TB/s), sum 114 us (5.3 TB/s), its backward 219 us (1.14 GB, 5.2 TB/s).
+// HBM-bound: every row is read once and written once. 8192 tokens x 8 x 4096 bf16, a random choice of 64 experts: sum 117 us
+// (604 MB, 5.2 TB/s), its backward 218 us (1.14 GB, 5.2 TB/s), gather 142 us (604 MB, 4.3 TB/s). What the L2s move for the last two is
+// more: a token's row is wanted by wavefronts of up to eight XCDs and fetched by each of their L2s, 496 MB of reads for 67 MB
+// of rows in the gather (7.2 TB/s with its writes), 810 MB in the backward (6.1 TB/s).
 #include <initializer_list>
 #include <type_traits>
 

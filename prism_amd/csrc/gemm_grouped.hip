@@ -14,10 +14,10 @@
 // they hold.
 //
 // 2 R N K flop. With many rows a group the matrix pipe bounds them, with few reading B (at 1.4 PFLOP/s and 6 TB/s both take as
-// long at some 230 rows). Three kernels (choose_kernel):
-// 16, 128 or 256 rows a tile. bf16, 2048 x 4096 matrices: forward 65536 rows of 64 groups 880 us (1.25 PFLOP/s; the dense
-// product of this library reaches 1.5), grad_a 32768 rows of 32 groups 478 us (1.15), grad_b of the same 606 us (0.91, and
-// 1.07 GB of fp32 results). 32 rows of 64 groups, 1536 x 2048, at most 160 MB of B: 30 us (5.3 TB/s).
+// long at some 230 rows). Three kernels (choose_kernel): 16, 128 or 256 rows a tile. Calls among others, three sets of inputs in
+// turn, 2048 x 4096 matrices: forward 65536 rows of 64 groups 890 to 910 us (1.22 PFLOP/s; the dense product of this library
+// reaches 1.5), grad_a 32768 rows of 32 groups 474 to 496 us (1.13), grad_b of the same 618 to 630 us (0.88, and 1.07 GB of fp32
+// results). 32 rows of 64 groups, 1536 x 2048, 160 MB of B: 30 to 32 us (5.1 TB/s).
 #include <type_traits>
 
 #include "common.h"
@@ -176,9 +176,10 @@ __device__ __forceinline__ void load_packets(uint16_t* tile, const OperandSource
 
 // ------------------------------------------------------------------------------------------- the general kernel --
 // 128 x 128 tiles, four waves of 64 x 64, one tile a workgroup: operands of any alignment, and problems with too few big
-// tiles for the chip. RAGGED_C: the groups lie along c (grad_b). Bound by what feeds the matrix pipe: a stage is 32 KiB into
-// LDS and 64 KiB out of it for 0.21 us of matrix instructions. 5003 rows of 24 groups by 1000 x 1048, fp32 results: 28.5 us
-// (0.37 PFLOP/s).
+// tiles for the chip. RAGGED_C: the groups lie along c (grad_b), whose rows one workgroup walks by itself: with few results that
+// leaves compute units idle (16384 rows of 4 groups by 256 x 256: 16 workgroups, 48 us; 65 with a long group among them). Bound by
+// the latency of its loads: a stage of two workgroups on a unit takes 1.1 us for 0.42 us of matrix instructions. 5003 rows of 24
+// groups by 1000 x 1048, fp32 results: 30 us a call (0.35 PFLOP/s; matrix pipe 19 % busy, 143 MB read for 61 of operands).
 // Direct-to-LDS loads into a ring of STAGES stages of 64 c. Four, three ahead, where there is a tile to a CU and nothing else
 // hides the memory's latency (with two stages, one ahead, a stage took 0.65 us, memory latency, instead of 0.45); two where
 // there are more tiles and two workgroups share a CU (choose_kernel). Not ALIGNED: the last stage, or every one of rows too
@@ -733,7 +734,7 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
 // The forward product where a group has few rows: reading B bounds it. A wavefront takes 16 columns and a slice of K, 128 k
 // to a step; its lane reads 16 B of the column's row of B for every instruction (the four lanes of a row 64 B, the next
 // instruction's the rest of the line), so the rows need no alignment. The parts of a column tile meet in LDS. 64 matrices of
-// 1536 x 2048, 32 rows: 30 us, 5.3 TB/s.
+// 1536 x 2048, 32 rows: 30 to 32 us a call, 5.1 TB/s.
 constexpr int kFewWaves = 8, kFewLeast = 2, kFewStep = 128;
 
 struct FewProblem {
@@ -885,7 +886,7 @@ int run_few(const GroupedProblem& g, const char* who, hipStream_t s) {
 }
 
 // Which kernel: the one with the smallest estimate, in us, of these simple costs (all figures measured on one MI355X with
-// 32 or fewer groups; `used` groups have rows, which the host takes to be as many as there can be, and a group wastes half a
+// 8 to 64 groups; `used` groups have rows, which the host takes to be as many as there can be, and a group wastes half a
 // row tile):
 //   few      5 + B read once per 16-row tile at 5.3 TB/s with up to 4 rows a group, 3.9 with more (see instruction_x)
 //   general  rounds of 256 tiles of 128 x 128 at 4 + 0.48 a stage with a ring of four stages, of 512 at 4 + 1.1 with one of

@@ -4,8 +4,7 @@
 //
 // Reading q bounds it: N K / 2 bytes for 2 r N K flop. The weights go from memory straight into registers, become bf16
 // there and are multiplied on the matrix cores (v_mfma_f32_16x16x32_bf16: 16 rows of x, padded with zeros, by 16
-// columns n, 32 k at a time), so that up to 16 rows cost what one costs. Three things keep the vector ALU out of the
-// way:
+// columns n, 32 k at a time), so that 16 rows share one unpacking. Three things keep the vector ALU out of the way:
 //   * the order of k inside an instruction is free as long as both operands have the same: a lane takes 16 consecutive
 //     bytes of its row (32 weights; where groups are shorter than the 128 of a row's four lanes, the lanes exchange dwords
 //     so that an instruction stays inside a group), and the values of a dword in the order 0 4 1 5 2 6 3 7, in which
@@ -15,10 +14,16 @@
 //     factor, taken back off the result, neither part overflows for any finite x (128 * 271 < 2^16) though x (q - z) does not,
 //     and products keep all their bits down to the smallest x (2^-133 2^-16 is fp32's smallest number);
 //   * the scale is applied to a group's fp32 sum, not to the weights. Nothing is rounded below 32 bits but the result.
-// Kernel times: 8192 x 8192, G = 128, 1 row: 9.8 us (34.6 MB, 3.5 TB/s); 16384 x 16384: 30.2 us (4.6 TB/s); 64 matrices of
-// 1536 x 2048, G = 32 with zero points, 32 rows: 17 us. What is left is latency: two rounds of loads in flight a wavefront, three to
-// six rounds a slice, and some 4 us in which the first weights arrive and the parts meet. x in LDS (+2 to 5 us), sixteen
-// wavefronts a workgroup, all of K up front and non-temporal loads (+1.4 us) were slower.
+// Calls back to back with the same weights every time, which the memory-side cache then holds, / with weights from memory: 8192 x
+// 8192, G = 128, 1 row: 10.0 / 12.0 us (34.6 MB, 2.9 TB/s); 16384 x 16384: 26.6 / 32 to 38 us (139 MB, 3.7 to 4.3 TB/s); 32 rows of 64
+// matrices 1536 x 2048, 26 of them used: 13.3 / 15.1 us with G = 128, 16.5 / 18.5 with G = 32, zero points and fp32 results. What is
+// left is latency: two rounds of loads in flight a wavefront, three to six rounds a slice, and some 4 us in which the first weights
+// arrive and the parts meet; 8 to 11 wavefronts a CU are there on average, of the 12 that the registers allow at G = 32 with zero
+// points (16 elsewhere, 8 to 12 at group sizes that are looked up). x in LDS (+2 to 5 us), sixteen wavefronts a workgroup,
+// all of K up front and non-temporal loads (+1.4 us) were slower.
+// Beyond four rows x counts: a tile of 16 columns reads 8 bytes of weights and 2 bytes a row of x for a k, x from the L2.
+// 8192 x 8192, G = 128, kernels by themselves: 1, 2, 4, 5, 8, 16 rows 11.7, 12.8, 14.1, 16.6, 18.8, 42.0 us; 64, 256, 2048 rows 94, 331, 2456 us,
+// since every 16 rows unpack all weights again.
 #include <type_traits>
 
 #include "common.h"
@@ -352,7 +357,7 @@ int launch_gemv_w4(int groups, long long rows, int N, int K, const uint16_t* x, 
     const long long row_tiles = offsets != nullptr ? most_row_tiles(rows, groups, 16) : ceil_div(rows, 16ll);
     const long long busy = offsets != nullptr ? busy_row_tiles(rows, groups, row_tiles) : row_tiles;
     // Twelve wavefronts a CU, none with less than a round of few rows (512 k: shorter slices only have the loop's last,
-    // unpipelined part). Against eight and single steps: 16384 x 16384 by 1 row 35.6 -> 30.2 us, 8192 x 1024 by 16 rows 7.1 -> 5.3,
+    // unpipelined part). Kernels by themselves with the same weights every time, against eight and single steps: 16384 x 16384 by 1 row 35.6 -> 30.2 us, 8192 x 1024 by 16 rows 7.1 -> 5.3,
     // 2048 x 1024 by 4 rows 5.0 -> 3.7, none of sixteen sizes slower by 1 %; sixteen wavefronts lose 40 % on
     // 14336 x 4096 by 1 row (9.1 -> 13.0 us) and 19 % on 8 matrices of 2048 x 2048 by 64 rows.
     p.k_parts = few_rows_k_parts(busy, N, K, 4 * kW4Block, kW4Waves, 12);

@@ -10,9 +10,13 @@
 //             offsets[e] entries go to experts below e, rows[s] is the entry in slot s, slots[t][j] its inverse.
 // Ranks come from counts and from positions inside a wavefront, never from the order in which atomics arrive.
 //
-// Launches and dependent steps bound it, not bytes. Router and plan: 1 token, 64 experts, k = 4: one kernel of 4.5 us (7.7 us
-// a call from Python); 16384 tokens, 256 experts bf16, k = 8: choice and counts 7.4 us (8.4 MB; eight rounds of a 16-lane
-// maximum), sums 3.3, places 5.8, together 14.7 us (bf16 keys struck out one by one and counts summed one by one: 17.2). Gradient of 32768 x 128 fp32: 8.3 us, 4.4 TB/s.
+// Launches and dependent steps bound it, not bytes. Router and plan, calls from C back to back: 1 token, 64 experts, k = 4:
+// 4.8 us, one kernel; 16384 tokens, 256 experts bf16, k = 8: 14.7 us (bf16 keys struck out one by one and counts summed one by
+// one: 17.2). Its kernels, each by itself in a trace: choice and counts 7.3 us (8.4 MB; eight rounds of a 16-lane maximum), sums
+// 3.4, places 5.8. Above 256 experts a lane holds 64 keys whatever their number, which costs where it is not near 1024: choice
+// and counts of 16384 bf16 tokens 12.6 us with 384 experts, 13.5 with 512, 16.3 with 1024; fp32 12.1 with 256, 27.9 with 384, 32.2 with
+// 1024 (128 registers, and 12 B of scratch in the form for rows of any alignment). Gradient of 32768 x 128 fp32: 8.2 us,
+// 4.5 TB/s.
 #include <cmath>
 #include <type_traits>
 

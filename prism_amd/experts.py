@@ -366,7 +366,7 @@ def gemv_w4(x: "torch.Tensor", q: "torch.Tensor", scales: "torch.Tensor", group_
     ceil(K / G)] bf16, zeros: the same shape, uint8 (None: 8 throughout). G = group_size, a multiple of 32. With offsets
     (int32, on the device) q, scales and zeros have a leading dimension, one weight matrix per group, and row r of group g
     uses matrix g, as in gemm_bf16_grouped. out: [R, N] bf16 or fp32 (a new one: of out_dtype); rows of no group are
-    left as they are. Sums are in fp32. Made for up to 16 rows a group.
+    left as they are. Sums are in fp32. Made for few rows a group: every 16 rows unpack the weights again.
     """
     ldx = _matrix(x, _BF16, "x")
     R, K = x.shape
