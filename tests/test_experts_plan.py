@@ -43,3 +43,15 @@ def test_empty_calls_and_refusals():
                               (lambda: prism.gemm_bf16_grouped_plan("forward", 1 << 40, 8, 8, 8), ValueError, "31 bits")):
         with pytest.raises(error, match=text):
             call()
+
+
+def test_calls_without_a_workspace_are_those_that_need_none():
+    """The Python calls know by themselves which plans need no workspace; the library must agree."""
+    from prism_amd import _lib, experts
+    lib, host = _lib.load(), torch.empty(0)
+    for tokens in (0, 1, 64, 65, 128, 511, 512, 513, 1024, 4095, 4096, 4097, 5000):
+        for k in (1, 2, 4, 8, 32):
+            for num in (1, 64, 511, 512, 513, 1024):
+                need, workspace = experts._plan_workspace(tokens, k, num, host)
+                bytes_ = lib.prism_expert_plan_workspace_bytes(tokens, k, num)
+                assert (need, workspace) == (0, None) if bytes_ == 16 else (need == bytes_ and workspace.numel() == bytes_), (tokens, k, num)
