@@ -17,7 +17,8 @@
 // long at some 230 rows). Three kernels (choose_kernel): 16, 128 or 256 rows a tile. Calls among others, three sets of inputs in
 // turn, 2048 x 4096 matrices: forward 65536 rows of 64 groups 890 to 910 us (1.22 PFLOP/s; the dense product of this library
 // reaches 1.5), grad_a 32768 rows of 32 groups 474 to 496 us (1.13), grad_b of the same 618 to 630 us (0.88, and 1.07 GB of fp32
-// results). 32 rows of 64 groups, 1536 x 2048, 160 MB of B: 30 to 32 us (5.1 TB/s).
+// results). 32 rows of 64 groups, 1536 x 2048, 160 MB of B: 30 to 36 us, box to box (4.5 to
+// 5.3 TB/s).
 #include <type_traits>
 
 #include "common.h"
@@ -734,7 +735,7 @@ __global__ __launch_bounds__(256) void gemm_grouped_big_kernel(GroupedProblem g)
 // The forward product where a group has few rows: reading B bounds it. A wavefront takes 16 columns and a slice of K, 128 k
 // to a step; its lane reads 16 B of the column's row of B for every instruction (the four lanes of a row 64 B, the next
 // instruction's the rest of the line), so the rows need no alignment. The parts of a column tile meet in LDS. 64 matrices of
-// 1536 x 2048, 32 rows: 30 to 32 us a call, 5.1 TB/s.
+// 1536 x 2048, 32 rows: 30 to 36 us a call, box to box, 4.5 to 5.3 TB/s.
 constexpr int kFewWaves = 8, kFewLeast = 2, kFewStep = 128;
 
 struct FewProblem {
