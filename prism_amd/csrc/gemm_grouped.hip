@@ -15,10 +15,9 @@
 //
 // 2 R N K flop. With many rows a group the matrix pipe bounds them, with few reading B (at 1.4 PFLOP/s and 6 TB/s both take as
 // long at some 230 rows). Three kernels (choose_kernel): 16, 128 or 256 rows a tile. Calls among others, three sets of inputs in
-// turn, 2048 x 4096 matrices: forward 65536 rows of 64 groups 890 to 910 us (1.22 PFLOP/s; the dense product of this library
-// reaches 1.5), grad_a 32768 rows of 32 groups 474 to 496 us (1.13), grad_b of the same 618 to 630 us (0.88, and 1.07 GB of fp32
-// results). 32 rows of 64 groups, 1536 x 2048, 160 MB of B: 30 to 36 us, box to box (4.5 to
-// 5.3 TB/s).
+// turn, from box to box, 2048 x 4096 matrices: forward 65536 rows of 64 groups 870 to 910 us (1.21 to 1.26 PFLOP/s; the dense
+// product of this library reaches 1.5), grad_a 32768 rows of 32 groups 470 to 496 us (1.11 to 1.17), grad_b of the same 613 to
+// 631 us (0.87 to 0.90, and 1.07 GB of fp32 results). 32 rows of 64 groups, 1536 x 2048, 160 MB of B: 30 to 36 us (4.5 to 5.3 TB/s).
 #include <type_traits>
 
 #include "common.h"
